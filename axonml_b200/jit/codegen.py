@@ -132,8 +132,8 @@ def generate_cuda(graph: Graph):
             continue
         else:
             expr = _EXPR[k].format(*a)
-        name_of[n.id] = f"v{n.id}"
-        body.append(f"    const float v{n.id} = {expr};")
+        name_of[n.id] = f"v{int(n.id)}"       # a node id prints with a percent sign
+        body.append(f"    const float {name_of[n.id]} = {expr};")
     src = ("extern \"C\" __global__ void axonml_fused(" + ", ".join(params) + ", long n) {\n"
            "  for (long i = (long)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (long)gridDim.x * blockDim.x) {\n"
            + "\n".join(body) + "\n  }\n}\n")

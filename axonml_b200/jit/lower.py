@@ -110,7 +110,7 @@ class _KernelBuilder:
         if nid in self.mat and not root:
             if nid not in self.leaves:
                 self.leaves.append(nid)
-            e = f"b{nid}[{idx}]" if _numel(n.shape) > 1 else f"b{nid}[0]"
+            e = f"b{int(nid)}[{idx}]" if _numel(n.shape) > 1 else f"b{int(nid)}[0]"
             self.memo[key] = e
             return e
         ins = n.op.inputs
@@ -194,7 +194,7 @@ class Plan:
                 self.steps.append({"kind": "matmul", "out": n.id, "a": n.op.inputs[0], "b": n.op.inputs[1]})
                 continue
             kb = _KernelBuilder(g, mat)
-            name = f"axonml_k{n.id}"
+            name = f"axonml_k{int(n.id)}"
             if k in _REDUCE:
                 x = g.node(n.op.inputs[0])
                 if k in ("Sum", "Mean"):
@@ -209,7 +209,7 @@ class Plan:
                 threads = 256 if red // split >= 2048 else 32
                 val = kb.value(x.id, "xl")
                 body = "\n      ".join(kb.stmts)
-                params = ", ".join([f"const float* __restrict__ b{l}" for l in kb.leaves] + ["float* __restrict__ out"])
+                params = ", ".join([f"const float* __restrict__ b{int(l)}" for l in kb.leaves] + ["float* __restrict__ out"])
                 comb = "fmaxf(acc, {0})" if is_max else "(acc + {0})"
                 init = "__int_as_float(0xff800000)" if is_max else "0.f"
                 scale = f" * {1.0 / red!r}f" if k in ("Mean", "MeanAxis") else ""
@@ -248,7 +248,7 @@ extern "C" __global__ void __launch_bounds__({threads}) {name}({params}) {{
             else:
                 val = kb.value(n.id, "lin", root=True)
                 body = "\n    ".join(kb.stmts)
-                params = ", ".join([f"const float* __restrict__ b{l}" for l in kb.leaves] + ["float* __restrict__ out", "long total"])
+                params = ", ".join([f"const float* __restrict__ b{int(l)}" for l in kb.leaves] + ["float* __restrict__ out", "long total"])
                 src.append(f"""
 extern "C" __global__ void __launch_bounds__(256) {name}({params}) {{
   for (long lin = (long)blockIdx.x * blockDim.x + threadIdx.x; lin < total; lin += (long)gridDim.x * blockDim.x) {{

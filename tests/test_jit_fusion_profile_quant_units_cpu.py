@@ -404,3 +404,32 @@ def test_quantisation_error_and_model_quantisation():
     assert st.max_error >= st.mean_error > 0 and st.rmse > 0 and st.compression_ratio == 8.0
     out = Q.quantize_model({"big": torch.randn(64, 64), "tiny": torch.randn(8)}, Q.QuantType.Q8_0)
     assert out["big"].quant_type is Q.QuantType.Q8_0 and out["tiny"].quant_type is Q.QuantType.F32            # small tensors stay exact
+
+
+def test_generated_elementwise_source_uses_valid_identifiers():
+    """Node ids print as ``%n``; the names in the generated CUDA must not contain that sign."""
+    from axonml_b200 import jit
+    from axonml_b200.jit.codegen import generate_cuda
+
+    def f(tr):
+        a, b = tr.input("a", [8]), tr.input("b", [8])
+        return tr.output("y", a.mul(b).add_scalar(0.5).tanh())
+    src, ins, outs, shape = generate_cuda(jit.trace(f))
+    assert "%" not in src and "const float v2 = (v0 * v1);" in src
+    assert ins == ["a", "b"] and outs == ["y"] and tuple(shape) == (8,)
+
+
+def test_lowered_plan_source_uses_valid_identifiers():
+    """The same for the multi-kernel plan: buffers and kernels are named by number."""
+    from axonml_b200 import jit
+    from axonml_b200.jit import lower
+
+    def f(tr):
+        a = tr.input("a", [4, 8])
+        return tr.output("y", a.mul_scalar(2.0).sum_axis(1, False))
+    g = jit.trace(f)
+    if not lower.lowerable(g):
+        pytest.fail("the graph should lower")
+    src = lower.Plan(g).source
+    assert "axonml_k" in src and "b0[" in src
+    assert "axonml_k%" not in src and "b%" not in src
