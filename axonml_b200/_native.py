@@ -63,6 +63,20 @@ class _CountingLib:
         return fn
 
 
+# Argument types of entry points that are called with plain Python numbers and addresses (p pointer,
+# i int, l long, f float): cheaper per call than wrapping every argument in a ctypes object.
+_SIGNATURES = {
+    "ax_int8_rows": "iiipl" "pl" "pf" "pl" "pl" "piip",
+    "ax_int8_gemm": "plp" "plp" "ppl" "iiiipp",
+}
+
+
+def _declare(lib) -> None:
+    kinds = {"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float}
+    for name, sig in _SIGNATURES.items():
+        getattr(lib, name).argtypes = [kinds[c] for c in sig]
+
+
 def bounds_build() -> bool:
     """``AXONML_BOUNDS=1`` selects the debug build of the kernels whose index checks report a wrong
     index (``bounds_report``) instead of using it."""
@@ -80,9 +94,11 @@ def cuda():
                     if not path.exists() or os.environ.get("AXONML_REBUILD") == "1":
                         from . import _build
                         _build.build_cuda(verbose=True, bounds=True)
-                    _CUDA = _CountingLib(ctypes.CDLL(str(path)))
+                    lib = ctypes.CDLL(str(path))
                 else:
-                    _CUDA = _CountingLib(_load("libaxonml_cuda.so", "build_cuda"))
+                    lib = _load("libaxonml_cuda.so", "build_cuda")
+                _declare(lib)
+                _CUDA = _CountingLib(lib)
     return _CUDA
 
 
@@ -159,6 +175,31 @@ class KernelTimeout(RuntimeError):
     def __init__(self, code: int, where: int, block: int):
         super().__init__(f"kernel status code={code} where={where} block={block}")
         self.code, self.where, self.block = code, where, block
+
+
+def launch(name: str, device: torch.device, *args) -> None:
+    """Calls entry point ``name`` of ``_SIGNATURES`` on ``device``'s current stream (its last argument),
+    also when that is not the current device, and raises on a non-zero code."""
+    fn = getattr(cuda(), name)
+    if device.index == torch._C._cuda_getDevice():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    else:
+        with torch.cuda.device(device):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    if rc != 0:
+        raise NativeError(f"{name} failed with code {rc}")
+
+
+def status_ptr(device: torch.device) -> int:
+    """Address of ``device``'s status word.  The word has to exist before a stream capture: made inside
+    one, it would be cleared by every replay."""
+    t = _STATUS.get(("cuda", device.index))
+    if t is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise NativeError("call the operator once before capturing it: its status word does not exist yet")
+        t = status_word(device)
+        torch.cuda.current_stream(device).synchronize()      # other streams use the word from now on
+    return t.data_ptr()
 
 
 def check_status(device=None) -> None:
