@@ -42,7 +42,8 @@ class _CountingLib:
     (every ``ax_*`` entry that takes a stream launches at least one kernel)."""
 
     _NO_LAUNCH = {"ax_version", "ax_sm_count", "ax_norm_bwd_groups", "ax_multi_tensor_limits", "ax_gemm_comm_set_trace",
-                  "ax_flash_fwd_set_trace", "ax_gemm_comm_signal_slots", "ax_norm_bwd_noalloc_limits", "ax_gemm_set_pair_mode", "ax_flash_fwd_set_one_tile", "ax_bounds_enabled", "ax_bounds_read", "ax_gemm_pair_capacity"}
+                  "ax_flash_fwd_set_trace", "ax_gemm_comm_signal_slots", "ax_norm_bwd_noalloc_limits", "ax_gemm_set_pair_mode", "ax_flash_fwd_set_one_tile", "ax_bounds_enabled", "ax_bounds_read", "ax_gemm_pair_capacity",
+                  "ax_decode_int8_workspace"}
 
     def __init__(self, lib):
         self._lib = lib
@@ -68,6 +69,9 @@ class _CountingLib:
 _SIGNATURES = {
     "ax_int8_rows": "iiipl" "pl" "pf" "pl" "pl" "piip",
     "ax_int8_gemm": "plp" "plp" "ppl" "iiiipp",
+    "ax_kv_write_int8": "i" "pll" "pll" "pppp" "ppp" "iiiiiii" "pp",
+    "ax_decode_int8": "ppp" "pppp" "p" "iiiiiii" "f" "ppp",
+    "ax_decode_int8_workspace": "iiiiii",
 }
 
 
@@ -75,6 +79,7 @@ def _declare(lib) -> None:
     kinds = {"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float}
     for name, sig in _SIGNATURES.items():
         getattr(lib, name).argtypes = [kinds[c] for c in sig]
+    lib.ax_decode_int8_workspace.restype = c_int64
 
 
 def bounds_build() -> bool:

@@ -1,0 +1,712 @@
+// Paged K/V cache in 8 bits: pages of P tokens, one magnitude a for each (page, KV head) of K and of V;
+// a stored byte q stands for q a / 127.
+//
+//   k_cache [pages, Hkv, P, D]            k_amax [pages, Hkv]
+//   v_cache [pages, Hkv, P / 16, D, 16]   v_amax [pages, Hkv]
+//
+// K keeps a token's dims side by side, V keeps sixteen tokens of one dim side by side: both are the order
+// in which the two matrix products contract (over dims, over tokens), so a lane's bytes become MMA
+// operands without a transposition, and sixteen tokens of a head are one contiguous 16 D byte piece of
+// either, which one bulk copy fetches.
+//
+// Writing: a page's magnitude grows to the largest it holds; what it held is scaled to the new one
+// (rint(q a_old / a_new)), new rows are rint(127 x / a).  A page written from its first slot starts anew.
+//
+// Attention of one query token per sequence: softmax(q K^T scale) V over the first ctx tokens.
+#include "int8_common.cuh"
+
+namespace {
+using namespace ax;
+
+// ------------------------------------------------------------------------------------ write
+struct WriteArgs {
+  const void *k, *v;          // [T, Hkv, D]
+  int8_t *kc, *vc;
+  float *ka, *va;
+  const int* table;           // [B, max_pages]
+  const int* starts;          // [B] position of the first new token
+  const int* cu;              // [B + 1] first token of each row in k / v, or null: T / B tokens each
+  long k_ts, k_hs, v_ts, v_hs;
+  int T, B, Hkv, D, P, max_pages, num_pages;
+  int* status;
+};
+
+struct Piece { int page, first, count, src; };   // slots [first, first + count) of a page, from token src
+
+// Pages touched by row b: 0 for an empty row or one that does not fit.
+__device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start, int& src, int& len) {
+  start = a.starts[b];
+  if (a.cu != nullptr) {
+    src = a.cu[b];
+    len = a.cu[b + 1] - src;
+  } else {
+    len = a.T / a.B;
+    src = b * len;
+  }
+  if (len <= 0) return 0;
+  if (start < 0 || src < 0 || src + len > a.T || (long)start + len > (long)a.max_pages * a.P) {
+    set_status(a.status, kBadArgument, 1200);
+    return 0;
+  }
+  return (start + len - 1) / a.P - start / a.P + 1;
+}
+
+// The piece that block `slot` of the grid works on: every warp walks the rows 32 at a time, adding up
+// their pages until it passes `slot`.
+__device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& out) {
+  const int lane = threadIdx.x & 31;
+  int base = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    int start = 0, src = 0, len = 0, n = 0;
+    if (b0 + lane < a.B) n = row_pieces(a, b0 + lane, start, src, len);
+    int upto = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += t;
+    }
+    const int total = __shfl_sync(0xffffffffu, upto, 31);
+    if (slot < base + total) {
+      const int own = __ffs(__ballot_sync(0xffffffffu, base + upto > slot)) - 1;
+      const int j = slot - base - (__shfl_sync(0xffffffffu, upto - n, own));
+      start = __shfl_sync(0xffffffffu, start, own);
+      src = __shfl_sync(0xffffffffu, src, own);
+      len = __shfl_sync(0xffffffffu, len, own);
+      const int idx = start / a.P + j;                       // which page of the row
+      const int lo = max(start, idx * a.P), hi = min(start + len, (idx + 1) * a.P);
+      out.page = a.table[(long)(b0 + own) * a.max_pages + idx];
+      out.first = lo - idx * a.P;
+      out.count = hi - lo;
+      out.src = src + lo - start;
+      if (out.page < 0 || out.page >= a.num_pages) { set_status(a.status, kBadArgument, 1201); return false; }
+      return true;
+    }
+    base += total;
+  }
+  return false;
+}
+
+__device__ __forceinline__ float elem(const float* p) { return *p; }
+__device__ __forceinline__ float elem(const __nv_bfloat16* p) { return __bfloat162float(*p); }
+__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
+  const uint4 u = *reinterpret_cast<const uint4*>(p);
+  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
+  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
+}
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+}
+
+// rint(q a_old / a_new); the same border rule as int8_step
+__device__ __forceinline__ int rescale_step(int q, float old, float grown, float ratio) {
+  const float f = (float)q * ratio;
+  float n = rintf(f);
+  if (!(fabsf(fabsf(f - n) - 0.5f) >= 1e-4f)) n = rintf(__fdiv_rn(__fmul_rn((float)q, old), grown));
+  return __float2int_rn(n);
+}
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, float grown, float ratio) {
+  return pack_int8x4(rescale_step((int8_t)(w & 255), old, grown, ratio), rescale_step((int8_t)((w >> 8) & 255), old, grown, ratio),
+                     rescale_step((int8_t)((w >> 16) & 255), old, grown, ratio), rescale_step((int8_t)(w >> 24), old, grown, ratio));
+}
+
+// Grid (pieces, Hkv, 2): one block per page piece and head of K (z = 0) or V (z = 1).  The new rows are
+// read twice, the second time from L1: once for the magnitude, once to be rounded.
+template <typename T>
+__global__ void __launch_bounds__(128) kv_write_int8_kernel(const WriteArgs a) {
+  __shared__ uint32_t s_top[4];
+  Piece pc;
+  if (!find_piece(a, (int)blockIdx.x, pc)) return;           // uniform over the block
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const bool is_v = blockIdx.z != 0;
+  const long ts = is_v ? a.v_ts : a.k_ts;
+  const T* x = (const T*)(is_v ? a.v : a.k) + (long)pc.src * ts + (long)h * (is_v ? a.v_hs : a.k_hs);
+  const long group = (long)pc.page * a.Hkv + h;
+  float* amax_p = (is_v ? a.va : a.ka) + group;
+  int8_t* dst = (is_v ? a.vc : a.kc) + group * a.P * a.D;
+
+  uint32_t top = 0;
+  const int per_row = a.D / 8;
+  for (int i = tid; i < pc.count * per_row; i += 128) {
+    const int t = i / per_row, c = (i - t * per_row) * 8;
+    float v[8];
+    load8(x + t * ts + c, v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+  }
+  const float before = pc.first > 0 ? *amax_p : 0.f;
+  top = __reduce_max_sync(0xffffffffu, top);
+  if (lane == 0) s_top[warp] = top;
+  __syncthreads();                                           // also: every thread has read the old magnitude
+  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+  const uint32_t old_bits = abs_bits(before) < kTinyBits ? 0u : abs_bits(before);
+  top = max(top, old_bits);
+  if (top < kTinyBits) top = 0;
+  const float grown = __uint_as_float(top), old = __uint_as_float(old_bits);
+  const float inv = top ? __fdiv_rn(127.f, grown) : 0.f;
+  const bool again = top > old_bits && pc.first > 0;
+  const float ratio = again ? __fdiv_rn(old, grown) : 1.f;
+  if (tid == 0) *amax_p = grown;
+
+  if (!is_v) {
+    if (again) {
+      uint2* rows = reinterpret_cast<uint2*>(dst);
+      for (int i = tid; i < pc.first * per_row; i += 128) {
+        const uint2 w = rows[i];
+        rows[i] = make_uint2(rescale4(w.x, old, grown, ratio), rescale4(w.y, old, grown, ratio));
+      }
+    }
+    for (int i = tid; i < pc.count * per_row; i += 128) {
+      const int t = i / per_row, c = (i - t * per_row) * 8;
+      float v[8];
+      load8(x + t * ts + c, v);
+      int s[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] = top ? int8_step(v[j], grown, inv) : 0;
+      *reinterpret_cast<uint2*>(dst + (long)(pc.first + t) * a.D + c) =
+          make_uint2(pack_int8x4(s[0], s[1], s[2], s[3]), pack_int8x4(s[4], s[5], s[6], s[7]));
+    }
+  } else {
+    // sixteen slots of one dim are one 16-byte word; slots that are neither old nor new keep their byte
+    const int g0 = again ? 0 : pc.first / 16, g1 = (pc.first + pc.count + 15) / 16, end = pc.first + pc.count;
+    for (int i = tid; i < (g1 - g0) * a.D; i += 128) {
+      const int g = g0 + i / a.D, d = i % a.D, s0 = g * 16;
+      uint4* p = reinterpret_cast<uint4*>(dst + (long)g * 16 * a.D + d * 16);
+      uint32_t w[4] = {0u, 0u, 0u, 0u};
+      if (s0 < pc.first || s0 + 16 > end) {
+        const uint4 o = *p;
+        w[0] = o.x; w[1] = o.y; w[2] = o.z; w[3] = o.w;
+      }
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const int slot = s0 + j;
+        int val = (int8_t)((w[j / 4] >> (8 * (j % 4))) & 255);
+        if (slot < pc.first) {
+          if (again) val = rescale_step(val, old, grown, ratio);
+        } else if (slot < end) {
+          val = top ? int8_step(elem(x + (slot - pc.first) * ts + d), grown, inv) : 0;
+        }
+        w[j / 4] = (w[j / 4] & ~(255u << (8 * (j % 4)))) | ((uint32_t)(val & 255) << (8 * (j % 4)));
+      }
+      *p = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
+// -------------------------------------------------------------------------------- attention
+// Every warp is a worker of its own: it takes an equal, contiguous share of all 16-token tiles of the
+// batch, counted over sequences, KV heads and tokens in that order, whatever the context lengths are.
+// Its tiles arrive in a ring of stages in shared memory, K and V of a tile by one bulk copy each, several
+// tiles ahead; page numbers and magnitudes of 32 tiles are fetched by the 32 lanes at once, a batch ahead.
+// The query heads of a KV head are the rows of mma.m16n8k16 (fp16 operands, fp32 sums):
+//   S[heads x 16] = Q K^T, then O[heads x D] = alpha O + a_v / 127 (P V)
+// int8 becomes fp16 exactly (byte | 0x6400 is 1024 + byte).  Q is scaled by a power of two to lie near one,
+// where fp16 holds every bf16 significand; P in [0, 1] is rounded to fp16 (2^-11), below bf16's own rounding
+// of the result.  A worker writes a head's result itself when all its tokens were in the worker's share,
+// and otherwise a partial (O, maximum, sum) that a second kernel merges.
+constexpr int kWarps = 4;
+constexpr int kTile = 16;
+
+struct AttnArgs {
+  const __nv_bfloat16* q;      // [B, Hq, D]
+  const int8_t *kc, *vc;
+  const float *ka, *va;
+  const int *table, *ctx;
+  __nv_bfloat16* out;          // [B, Hq, D]
+  float* part;                 // [workers][2][HG][D]
+  float* ml;                   // [workers][2][HG][2]
+  int B, Hq, Hkv, G, nblk, P, max_pages, num_pages, min_chunk, workers;
+  float scale_log2;            // scale * log2(e) / 127
+  int* status;
+};
+
+__device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) {
+  int n = a.ctx[b];
+  const long cap = (long)a.max_pages * a.P;
+  if (n < 0 || n > cap) {
+    set_status(a.status, kBadArgument, 1210);
+    n = n < 0 ? 0 : (int)cap;
+  }
+  return (n + kTile - 1) / kTile;
+}
+__device__ __forceinline__ int chunk_of(const AttnArgs& a, int total) {
+  const int even = (total + a.workers - 1) / a.workers;
+  return even > a.min_chunk ? even : a.min_chunk;
+}
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+               "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+               : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Four int8 to two fp16 pairs: the byte with its sign bit flipped is value + 128; over 0x64 it is 1024 + that.
+__device__ __forceinline__ void int8x4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  w ^= 0x80808080u;
+  const uint32_t l = __byte_perm(w, 0x64646464u, 0x4140), h = __byte_perm(w, 0x64646464u, 0x4342);
+  const __half2 off = __half2half2(__ushort_as_half((unsigned short)0x6480));   // 1152
+  const __half2 a = __hsub2(*reinterpret_cast<const __half2*>(&l), off), b = __hsub2(*reinterpret_cast<const __half2*>(&h), off);
+  lo = *reinterpret_cast<const uint32_t*>(&a);
+  hi = *reinterpret_cast<const uint32_t*>(&b);
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int D>
+struct AttnCfg {
+  static constexpr int kStage = 2 * kTile * D;                   // K and V of a tile
+  static constexpr int kStages = D == 64 ? 8 : (D == 128 ? 4 : 3);
+  static constexpr int kRing = kWarps * kStages * kStage;
+  static constexpr int kBlocks = D == 256 ? 2 : 3;               // blocks per SM that registers and shared memory allow
+};
+
+template <int D, int HG>
+__global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_kernel(const AttnArgs a) {
+  using C = AttnCfg<D>;
+  constexpr int NJ = D / 64;                                     // 64-dim groups: a lane's 16-byte pieces of a K row
+  constexpr int NT = D / 8;                                      // 8-dim tiles of O
+  constexpr int R = HG / 8;                                      // rows of the MMA a lane owns
+  extern __shared__ __align__(128) uint8_t smem[];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up; it waits for this grid's end
+  uint64_t* bars = (uint64_t*)(smem + C::kRing);
+  volatile int* dead = (volatile int*)(bars + kWarps * C::kStages);
+  int* prefix = (int*)(bars + kWarps * C::kStages) + 2;          // [B + 1] tiles of the sequences before
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    *dead = 0;
+    for (int i = 0; i < kWarps * C::kStages; ++i) mbar_init(&bars[i], 1);
+    mbar_fence_init();
+  }
+  if (warp == 0) {
+    int sum = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
+      int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, n, o);
+        if (lane >= o) n += t;
+      }
+      if (b0 + lane < a.B) prefix[b0 + lane + 1] = sum + n;
+      sum += __shfl_sync(0xffffffffu, n, 31);
+    }
+    if (lane == 0) prefix[0] = 0;
+  }
+  __syncthreads();
+  const int VH = a.Hkv * a.nblk;
+  const int total = prefix[a.B] * VH, chunk = chunk_of(a, total);
+  const int w = warp * (int)gridDim.x + (int)blockIdx.x;         // neighbouring workers on different SMs
+  const long f0l = (long)w * chunk;
+  if (f0l >= total) return;
+  const int f0 = (int)f0l, f1 = min(total, f0 + chunk), n = f1 - f0;
+  uint8_t* ring = smem + warp * C::kStages * C::kStage;
+  uint64_t* full = bars + warp * C::kStages;
+
+  // sequence whose tiles (times VH) contain flat tile f
+  auto find_seq = [&](int f) {
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid + 1] * VH > f) hi = mid; else lo = mid + 1;
+    }
+    return lo;
+  };
+  // what lane l knows about tile (batch + l): where its bytes lie, and its magnitudes
+  auto load_ids = [&](int t0, long& off, int& group) {
+    off = -1;
+    group = -1;
+    if (t0 + lane < n) {
+      const int f = f0 + t0 + lane, b = find_seq(f), tb = prefix[b + 1] - prefix[b], r = f - prefix[b] * VH;
+      const int vh = r / tb, tok = (r - vh * tb) * kTile;
+      const int page = a.table[(long)b * a.max_pages + tok / a.P];
+      if (page < 0 || page >= a.num_pages) {
+        set_status(a.status, kBadArgument, 1211);
+      } else {
+        group = page * a.Hkv + vh / a.nblk;
+        off = ((long)group * a.P + tok % a.P) * D;
+      }
+    }
+  };
+  auto load_amax = [&](int group, float& ka, float& va) {
+    ka = group >= 0 ? a.ka[group] : 0.f;
+    va = group >= 0 ? a.va[group] : 0.f;
+  };
+  long off_c, off_n = -1;
+  int grp_c, grp_n = -1;
+  float ka_c, va_c, ka_n = 0.f, va_n = 0.f;
+  load_ids(0, off_c, grp_c);
+  load_amax(grp_c, ka_c, va_c);
+  auto issue = [&](int t, long off) {                            // tile t of this worker into its stage
+    if (lane == 0) {
+      const int s = t % C::kStages;
+      if (off < 0) {
+        mbar_arrive(&full[s]);                                   // no such page: nothing is fetched, the tile is masked
+      } else {
+        uint8_t* dst = ring + s * C::kStage;
+        mbar_expect_tx(&full[s], C::kStage);
+        bulk_load(dst, a.kc + off, kTile * D, &full[s]);
+        bulk_load(dst + kTile * D, a.vc + off, kTile * D, &full[s]);
+      }
+    }
+  };
+#pragma unroll 1
+  for (int t = 0; t < C::kStages && t < n; ++t) issue(t, __shfl_sync(0xffffffffu, off_c, t));
+
+  const int g = lane >> 2, i4 = lane & 3;
+  int b = find_seq(f0), tb = prefix[b + 1] - prefix[b];
+  int vh = (f0 - prefix[b] * VH) / tb, tile = f0 - prefix[b] * VH - vh * tb;
+  int ctx = 0;
+  uint32_t qa[NJ * 4][2 * R];
+  float qs[R], m[R], l[R], o[NT][2 * R];
+  bool fresh = true;
+
+#pragma unroll 1
+  for (int t = 0; t < n; ++t) {
+    const int bi = t & 31;
+    if (bi == 0) {
+      if (t > 0) { off_c = off_n; grp_c = grp_n; ka_c = ka_n; va_c = va_n; }
+      if (t + 32 < n) load_ids(t + 32, off_n, grp_n);
+    }
+    if (bi == 8 && t - 8 + 32 < n) load_amax(grp_n, ka_n, va_n);
+    if (fresh) {
+      fresh = false;
+      ctx = min(a.ctx[b], a.max_pages * a.P);
+      const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        const bool live = first + g + 8 * r < a.G;
+        const __nv_bfloat16* qp = a.q + ((long)b * a.Hq + h0 + first + g + 8 * r) * D;
+        float v[NJ][16];
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          float x0[8], x1[8];
+          if (live) {
+            load8(qp + (i4 + 4 * j) * 16, x0);
+            load8(qp + (i4 + 4 * j) * 16 + 8, x1);
+          }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            v[j][e] = live ? x0[e] : 0.f;
+            v[j][8 + e] = live ? x1[e] : 0.f;
+            top = fmaxf(top, fmaxf(fabsf(v[j][e]), fabsf(v[j][8 + e])));
+          }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the power of two at or below the row's largest value (clamped: its inverse is a normal number too)
+        const uint32_t e = min(max(__float_as_uint(top) >> 23, 2u), 252u);
+        qs[r] = __uint_as_float(e << 23) * a.scale_log2;
+        const float down = __uint_as_float((254u - e) << 23);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            qa[j * 4 + k][r] = pack_half2(v[j][4 * k] * down, v[j][4 * k + 1] * down);
+            qa[j * 4 + k][R + r] = pack_half2(v[j][4 * k + 2] * down, v[j][4 * k + 3] * down);
+          }
+        m[r] = -INFINITY;
+        l[r] = 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int y = 0; y < 2 * R; ++y) o[x][y] = 0.f;
+    }
+    const int s = t % C::kStages;
+    bool ok = mbar_wait(&full[s], (uint32_t)((t / C::kStages) & 1), dead, a.status, 1212);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok) break;
+    const uint8_t* kt = ring + s * C::kStage;
+    const uint8_t* vt = kt + kTile * D;
+    const float ka = __shfl_sync(0xffffffffu, ka_c, bi), va = __shfl_sync(0xffffffffu, va_c, bi) * (1.f / 127.f);
+    const bool have = __shfl_sync(0xffffffffu, grp_c, bi) >= 0;
+    const int left = have ? ctx - tile * kTile : 0;              // tokens of the tile that count
+
+    // ---- S: column c of 8-token tile nt is token 4 (c / 2) + c % 2 + 2 nt, so that the lane's four scores are tokens 4 i4 ..
+    float sc[2][4];
+#pragma unroll
+    for (int nt = 0; nt < 2; ++nt) {
+      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
+      const uint8_t* row = kt + (4 * (g >> 1) + (g & 1) + 2 * nt) * D;
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint4 kk = *reinterpret_cast<const uint4*>(row + (i4 + 4 * j) * 16);
+        const uint32_t kw[4] = {kk.x, kk.y, kk.z, kk.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t b0, b1;
+          int8x4_to_half(kw[k], b0, b1);
+          const int x = j * 4 + k;
+          if (R == 1) mma_f16(sc[nt], qa[x][0], 0u, qa[x][1], 0u, b0, b1);
+          else mma_f16(sc[nt], qa[x][0], qa[x][1], qa[x][R], qa[x][R + (R - 1)], b0, b1);
+        }
+      }
+    }
+    // ---- running maximum and sum
+    uint32_t pa[2][2];                                           // [row][tokens 4 i4, +1 | +2, +3]
+    float alpha[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const float f = ka * qs[r];
+      float sv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sv[j] = 4 * i4 + j < left ? sc[j >> 1][2 * r + (j & 1)] * f : -INFINITY;
+      float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+      const float mn = fmaxf(m[r], mx);
+      const float base = mn == -INFINITY ? 0.f : mn;             // nothing seen yet: all weights are exp2(-inf) = 0
+      alpha[r] = exp2f(m[r] - base);
+      float pv[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) pv[j] = exp2f(sv[j] - base);
+      l[r] = l[r] * alpha[r] + (pv[0] + pv[1]) + (pv[2] + pv[3]);
+      m[r] = mn;
+      pa[r][0] = pack_half2(pv[0], pv[1]);
+      pa[r][1] = pack_half2(pv[2], pv[3]);
+    }
+    // ---- O
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      uint32_t b0, b1;
+      int8x4_to_half(*reinterpret_cast<const uint32_t*>(vt + (x * 8 + g) * 16 + i4 * 4), b0, b1);
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
+      mma_f16(c, pa[0][0], R == 2 ? pa[R - 1][0] : 0u, pa[0][1], R == 2 ? pa[R - 1][1] : 0u, b0, b1);
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        o[x][2 * r] = o[x][2 * r] * alpha[r] + c[2 * r] * va;
+        o[x][2 * r + 1] = o[x][2 * r + 1] * alpha[r] + c[2 * r + 1] * va;
+      }
+    }
+    __syncwarp();                                                // the stage has been read by all lanes
+    if (t + C::kStages < n) {
+      const int ahead = bi + C::kStages;
+      const long oc = __shfl_sync(0xffffffffu, off_c, ahead & 31), on = __shfl_sync(0xffffffffu, off_n, ahead & 31);
+      issue(t + C::kStages, ahead < 32 ? oc : on);
+    }
+    // ---- end of this head's tokens, or of this worker's share
+    if (tile + 1 == tb || t + 1 == n) {
+      const int seg = prefix[b] * VH + vh * tb;                  // flat tile the head begins with
+      const bool whole = seg >= f0 && seg + tb <= f1;
+      const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
+        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
+        const int head = first + g + 8 * r;
+        if (head < a.G) {
+          if (whole) {
+            const float inv = l[r] != 0.f ? __fdividef(1.f, l[r]) : 0.f;
+            __nv_bfloat16* op = a.out + ((long)b * a.Hq + h0 + head) * D + 2 * i4;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) *reinterpret_cast<uint32_t*>(op + x * 8) = pack_bf16x2(o[x][2 * r] * inv, o[x][2 * r + 1] * inv);
+          } else {
+            const long slot = ((long)w * 2 + (seg < f0 ? 0 : 1)) * HG + g + 8 * r;
+            float* pp = a.part + slot * D + 2 * i4;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) *reinterpret_cast<float2*>(pp + x * 8) = make_float2(o[x][2 * r], o[x][2 * r + 1]);
+            if (i4 == 0) { a.ml[slot * 2] = m[r]; a.ml[slot * 2 + 1] = l[r]; }
+          }
+        }
+      }
+    }
+    // ---- next tile: the next token block, KV head or non-empty sequence
+    if (++tile == tb) {
+      tile = 0;
+      fresh = true;
+      if (++vh == VH) {
+        vh = 0;
+        do { ++b; } while (b < a.B && prefix[b + 1] == prefix[b]);
+        if (b < a.B) tb = prefix[b + 1] - prefix[b];
+      }
+    }
+  }
+}
+
+// One block per query head: adds up the partials of a head whose tokens went to several workers, and
+// writes zeros for an empty context.  Its warps take the partials in turn; a lane holds D / 32 dims.
+template <int D, int HG>
+__global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
+  constexpr int E = D / 32;
+  extern __shared__ float smem_f[];                              // [warps][D] + [warps][2]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  const int b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
+  const int h = hq / a.G, hg = hq % a.G, vh = h * a.nblk + hg / HG, row = hg % HG;
+  const int VH = a.Hkv * a.nblk;
+  int before = 0, total = 0, tb = 0;
+  for (int b0 = 0; b0 < a.B; b0 += 32) {
+    const int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
+    total += n;
+    if (b0 + lane < b) before += n;
+    if (b0 + lane == b) tb = n;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    before += __shfl_xor_sync(0xffffffffu, before, o);
+    total += __shfl_xor_sync(0xffffffffu, total, o);
+    tb += __shfl_xor_sync(0xffffffffu, tb, o);
+  }
+  __nv_bfloat16* op = a.out + ((long)b * a.Hq + hq) * D;
+  asm volatile("griddepcontrol.wait;" ::: "memory");             // the first kernel is done, its partials are visible
+  if (tb == 0) {
+    if (warp == 0)
+      for (int d = lane; d < D; d += 32) op[d] = __float2bfloat16(0.f);
+    return;
+  }
+  const int chunk = chunk_of(a, total * VH), seg = before * VH + vh * tb;
+  const int w0 = seg / chunk, w1 = (seg + tb - 1) / chunk;
+  if (w0 == w1) return;                                          // one worker had it all and wrote it
+  float M = -INFINITY;
+  float acc[E], L = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+#pragma unroll 4
+  for (int x = w0 + warp; x <= w1; x += warps) {
+    const long slot = ((long)x * 2 + (x == w0 ? 1 : 0)) * HG + row;
+    const float ms = a.ml[slot * 2], ls = a.ml[slot * 2 + 1];
+    float v[E];
+    const float* pp = a.part + slot * D + lane * E;
+#pragma unroll
+    for (int e = 0; e < E; e += 2) {
+      const float2 t = *reinterpret_cast<const float2*>(pp + e);
+      v[e] = t.x; v[e + 1] = t.y;
+    }
+    const float mn = fmaxf(M, ms), base = mn == -INFINITY ? 0.f : mn;
+    const float fa = exp2f(M - base), fb = exp2f(ms - base);
+    L = L * fa + ls * fb;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = acc[e] * fa + v[e] * fb;
+    M = mn;
+  }
+  if (warps > 1) {
+    float* so = smem_f;
+    float* sm = smem_f + warps * D;
+#pragma unroll
+    for (int e = 0; e < E; ++e) so[warp * D + lane * E + e] = acc[e];
+    if (lane == 0) { sm[2 * warp] = M; sm[2 * warp + 1] = L; }
+    __syncthreads();
+    if (warp != 0) return;
+    const float mw = lane < warps ? sm[2 * lane] : -INFINITY;
+    M = warp_max(mw);
+    const float base = M == -INFINITY ? 0.f : M;
+    const float f = exp2f(mw - base);
+    L = warp_sum(lane < warps ? sm[2 * lane + 1] * f : 0.f);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = 0.f;
+    for (int x = 0; x < warps; ++x) {
+      const float fx = __shfl_sync(0xffffffffu, f, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += so[x * D + lane * E + e] * fx;
+    }
+  }
+  const float inv = L != 0.f ? __fdividef(1.f, L) : 0.f;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(op + lane * E + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, int HG>
+int launch_attn(AttnArgs& a, int blocks, int merge_warps, cudaStream_t stream) {
+  using C = AttnCfg<D>;
+  auto kern = decode_int8_kernel<D, HG>;
+  const int smem = C::kRing + kWarps * C::kStages * 8 + 8 + (a.B + 1) * 4;
+  static int configured[64] = {0};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || configured[dev] < smem) {
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return (int)e;
+    if (dev >= 0 && dev < 64) configured[dev] = smem;
+  }
+  kern<<<blocks, kWarps * 32, smem, stream>>>(a);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return (int)e;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the merge's own set-up runs beside the first kernel's end
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(a.B * a.Hq, 1, 1);
+  cfg.blockDim = dim3(32 * merge_warps, 1, 1);
+  cfg.dynamicSmemBytes = merge_warps * (D + 2) * 4;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return (int)cudaLaunchKernelEx(&cfg, merge_int8_kernel<D, HG>, a);
+}
+
+}  // namespace
+
+// New K/V rows [T, Hkv, D] (dt 1 bf16, 0 fp32; inner stride 1, token and head strides in elements, rows on 16-byte
+// boundaries) of B sequences into their pages.  Row b brings tokens cu[b] .. cu[b + 1] (cu null: T / B each) at positions
+// starts[b], starts[b] + 1, ...  Tokens behind cu[B] are not read.  A row that does not fit its table, or a page number outside
+// the cache, is recorded in `status` and skipped.
+AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const void* v, long v_ts, long v_hs, int8_t* kc, int8_t* vc,
+                            float* ka, float* va, const int* table, const int* starts, const int* cu, int T, int B, int Hkv, int D, int P,
+                            int max_pages, int num_pages, int* status, cudaStream_t stream) {
+  if (T <= 0 || B <= 0 || Hkv <= 0) return 0;
+  if (D % 8 || P % 16 || P <= 0 || Hkv > 65535 || (cu == nullptr && T % B)) return -1;
+  const int vec = dt == 1 ? 8 : 4;
+  if ((k_ts % vec) || (k_hs % vec) || (v_ts % vec) || (v_hs % vec) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)) return -2;
+  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, status};
+  // a row of n tokens touches at most (n - 1) / P + 2 pages; a single token one
+  const long rows = B < T ? B : T;
+  const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
+  const dim3 grid((unsigned)pieces, Hkv, 2);
+  if (dt == 1) kv_write_int8_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a);
+  else kv_write_int8_kernel<float><<<grid, 128, 0, stream>>>(a);
+  return (int)cudaGetLastError();
+}
+
+// Workers (warps) the attention kernel runs with: what fills the device, fewer for a small cache.
+static int attn_blocks(int B, int VH, int D, int max_pages, int P, int min_chunk) {
+  const long tiles = (long)B * VH * ((long)max_pages * P / kTile);
+  const long want = (tiles + (long)min_chunk * kWarps - 1) / ((long)min_chunk * kWarps);
+  const long most = (long)axh::sm_count() * (D == 256 ? 2 : 3);
+  const long few = (tiles + min_chunk - 1) / min_chunk;           // one worker a block while that spreads them further
+  const long n = want < axh::sm_count() ? (few < axh::sm_count() ? few : axh::sm_count()) : want;
+  return (int)(n < most ? (n > 0 ? n : 1) : most);
+}
+
+constexpr int kMinChunk = 4;
+
+// Floats of workspace that ax_decode_int8 needs (0: an argument it refuses).
+AX_API long ax_decode_int8_workspace(int B, int Hq, int Hkv, int D, int max_pages, int P) {
+  if (Hkv <= 0 || Hq % Hkv || P <= 0) return 0;
+  const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
+  const long workers = (long)attn_blocks(B, Hkv * nblk, D, max_pages, P, kMinChunk) * kWarps;
+  return workers * 2 * HG * (D + 2);
+}
+
+// out[B, Hq, D] = attention of q[B, Hq, D] (bf16, contiguous) over the first ctx[b] tokens of each sequence.
+// D in {64, 128, 256}; P a multiple of 16.  A context longer than the table and a page number outside the cache are
+// recorded in `status`; such tokens do not count.
+AX_API int ax_decode_int8(const void* q, const int8_t* kc, const int8_t* vc, const float* ka, const float* va, const int* table,
+                          const int* ctx, void* out, int B, int Hq, int Hkv, int D, int P, int max_pages, int num_pages, float scale,
+                          float* workspace, int* status, cudaStream_t stream) {
+  if (B <= 0) return 0;
+  if (Hkv <= 0 || Hq % Hkv || P <= 0 || P % 16 || B > 8192 || (long)B * Hq > 0x7fffffffL) return -1;
+  if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)workspace) & 15) return -2;
+  const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
+  if ((long)B * Hkv * nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv > 0x7fffffffL) return -3;
+  const int blocks = attn_blocks(B, Hkv * nblk, D, max_pages, P, kMinChunk);
+  const int workers = blocks * kWarps;
+  AttnArgs a{(const __nv_bfloat16*)q, kc, vc, ka, va, table, ctx, (__nv_bfloat16*)out, workspace, workspace + (long)workers * 2 * HG * D,
+             B, Hq, Hkv, G, nblk, P, max_pages, num_pages, kMinChunk, workers, scale * 1.4426950408889634f / 127.f, status};
+  // partials per head: many when few heads share all workers
+  const long heads = (long)B * Hkv * nblk, per = workers / (heads > 0 ? heads : 1) + 1;
+  const int mw = per <= 2 ? 1 : (per <= 8 ? 4 : (per <= 32 ? 8 : 16));
+#define AX_ATTN(DD)                                                      \
+  return HG == 8 ? launch_attn<DD, 8>(a, blocks, mw, stream) : launch_attn<DD, 16>(a, blocks, mw, stream)
+  switch (D) {
+    case 64: AX_ATTN(64);
+    case 128: AX_ATTN(128);
+    case 256: AX_ATTN(256);
+    default: return -4;
+  }
+#undef AX_ATTN
+}

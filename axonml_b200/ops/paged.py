@@ -1,5 +1,6 @@
 """Paged KV cache kernels (``csrc/kernels/paged_attn.cu``): scatter new K/V rows into pages, decode
-attention through a block table.  CPU tensors use the same maths with torch ops."""
+attention through a block table; the same over a cache held in int8 with one magnitude for each page
+and head (``csrc/kernels/paged_int8.cu``).  CPU tensors use the same maths with torch ops."""
 from __future__ import annotations
 
 import math
@@ -59,3 +60,160 @@ def decode_attention(q, k_cache, v_cache, block_table, ctx_lens, page_size: int,
         s = torch.einsum("hd,nhd->hn", q[b].float(), kk) * scale
         outs.append(torch.einsum("hn,nhd->hd", torch.softmax(s, -1), vv))
     return torch.stack(outs).to(q.dtype)
+
+
+# ------------------------------------------------------------------------------ cache in 8 bits
+def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
+    """``(pages, Hkv, page_size, D)`` of a consistent int8 cache."""
+    if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
+        raise TypeError("the caches must be int8")
+    if k_cache.dim() != 4:
+        raise ValueError(f"k_cache must be [pages, Hkv, page_size, D], not {tuple(k_cache.shape)}")
+    pages, Hkv, P, D = k_cache.shape
+    if P % 16 or P == 0 or D % 16 or D == 0:
+        raise ValueError(f"page_size {P} and head_dim {D} must be multiples of 16")
+    if v_cache.shape != (pages, Hkv, P // 16, D, 16):
+        raise ValueError(f"v_cache must be [pages, Hkv, page_size / 16, D, 16], not {tuple(v_cache.shape)}")
+    if k_amax.shape != (pages, Hkv) or v_amax.shape != (pages, Hkv):
+        raise ValueError(f"k_amax and v_amax must be [pages, Hkv] = {(pages, Hkv)}")
+    if k_amax.dtype != torch.float32 or v_amax.dtype != torch.float32:
+        raise TypeError("k_amax and v_amax must be fp32")
+    if block_table.dim() != 2 or block_table.dtype != torch.int32:
+        raise TypeError("block_table must be int32 [B, max_pages]")
+    for t in (k_cache, v_cache, k_amax, v_amax):
+        if not t.is_contiguous():
+            raise ValueError("the caches and their magnitudes must be contiguous")
+    for t in (v_cache, k_amax, v_amax, block_table):
+        if t.device != k_cache.device:
+            raise ValueError("the caches, their magnitudes and the block table must be on one device")
+    return pages, Hkv, P, D
+
+
+def _int32_vector(t, n: int, name: str, device):
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device:
+        raise ValueError(f"{name} must be int32 [{n}] on {device}")
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens=None) -> None:
+    """Writes new K/V rows ``[T, Hkv, D]`` (bf16 or fp32) into an int8 cache, in place.
+
+    ``k_cache`` is ``[pages, Hkv, page_size, D]``, ``v_cache`` ``[pages, Hkv, page_size / 16, D, 16]``, and a
+    stored ``q`` of page ``p``, head ``h`` stands for ``q * amax[p, h] / 127``.  Sequence ``b`` (a row of
+    ``block_table`` ``[B, max_pages]``) brings tokens ``cu_seqlens[b] .. cu_seqlens[b + 1]`` (without
+    ``cu_seqlens``: ``T / B`` each) at positions ``starts[b], starts[b] + 1, ...``; rows of ``k`` / ``v`` behind
+    ``cu_seqlens[B]`` are ignored.  A page's magnitude grows to the largest value it holds, and what it held
+    before is rounded to the new grid; a page written from its first slot starts anew.  Two sequences
+    of one call must not write to the same page.  On a GPU a sequence that does not fit its table or a
+    page number outside the cache is skipped and reported by ``_native.check_status()``."""
+    pages, Hkv, P, D = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
+    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+        raise ValueError(f"k and v must be [T, {Hkv}, {D}] of one type, not {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
+    if k.device != k_cache.device or v.device != k_cache.device:
+        raise ValueError("k and v must be on the cache's device")
+    T, B = k.shape[0], block_table.shape[0]
+    starts = _int32_vector(starts, B, "starts", k.device)
+    if cu_seqlens is not None:
+        cu_seqlens = _int32_vector(cu_seqlens, B + 1, "cu_seqlens", k.device)
+    elif B == 0 or T % B:
+        raise ValueError(f"without cu_seqlens, {T} tokens must divide evenly over {B} sequences")
+    if not k.is_cuda:
+        _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens)
+        return
+    if k.dtype not in (torch.bfloat16, torch.float32):
+        raise TypeError(f"k and v must be bf16 or fp32 on a GPU, not {k.dtype}")
+    if T == 0 or B == 0:
+        return
+    vec = 16 // k.element_size()
+    k, v = (t if t.stride(2) == 1 and t.stride(0) % vec == 0 and t.stride(1) % vec == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
+            for t in (k, v))
+    table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    N.launch("ax_kv_write_int8", k.device, int(k.dtype == torch.bfloat16), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+             v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(), v_amax.data_ptr(), table.data_ptr(), starts.data_ptr(),
+             cu_seqlens.data_ptr() if cu_seqlens is not None else 0, T, B, Hkv, D, P, table.shape[1], pages, N.status_ptr(k.device))
+
+
+def _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens) -> None:
+    T, B, P, D = k.shape[0], block_table.shape[0], k_cache.shape[2], k_cache.shape[3]
+    cu = cu_seqlens.tolist() if cu_seqlens is not None else [b * (T // B) for b in range(B + 1)]
+    table = block_table.tolist()
+    for b, start in enumerate(starts.tolist()):
+        n = cu[b + 1] - cu[b]
+        if n <= 0:
+            continue
+        if start < 0 or cu[b] < 0 or cu[b + 1] > T or start + n > block_table.shape[1] * P:
+            raise ValueError(f"sequence {b}: tokens {cu[b]}..{cu[b + 1]} at position {start} do not fit")
+        if any(not 0 <= p < k_cache.shape[0] for p in table[b][start // P:(start + n - 1) // P + 1]):
+            raise ValueError(f"sequence {b}: the block table names a page outside the cache")
+        pos = start
+        while pos < start + n:
+            page, lo = table[b][pos // P], pos % P
+            cnt = min(P - lo, start + n - pos)
+            src = cu[b] + pos - start
+            for x, cache, amax, is_v in ((k, k_cache, k_amax, False), (v, v_cache, v_amax, True)):
+                rows = cache[page].transpose(-1, -2).reshape(-1, P, D).clone() if is_v else cache[page]
+                new = x[src:src + cnt].transpose(0, 1).float()
+                old = amax[page].clone() if lo else torch.zeros_like(amax[page])
+                grown = torch.maximum(old, new.abs().amax((1, 2)))
+                one = torch.where(grown > 0, grown, torch.ones_like(grown))[:, None, None]
+                if lo:
+                    kept = (rows[:, :lo].float() * old[:, None, None] / one).round().nan_to_num_(0.0).to(torch.int8)
+                    rows[:, :lo] = torch.where((grown > old)[:, None, None], kept, rows[:, :lo])
+                rows[:, lo:lo + cnt] = (new * 127.0 / one).round().nan_to_num_(0.0).to(torch.int8)
+                amax[page] = grown
+                if is_v:
+                    cache[page] = rows.view(-1, P // 16, 16, D).transpose(-1, -2)
+            pos += cnt
+
+
+def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale: float | None = None):
+    """Attention of one query token per sequence over an int8 cache (laid out as ``kv_write_int8``
+    says): ``q`` bf16 ``[B, Hq, D]`` -> ``[B, Hq, D]``, each sequence over its first ``ctx_lens[b]`` tokens; an
+    empty context gives zeros.  On a GPU D is 64, 128 or 256; any number of query heads per KV head.  A
+    page number outside the cache and a context longer than the table are reported by
+    ``_native.check_status()`` and not read."""
+    pages, Hkv, P, D = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
+    if q.dim() != 3 or q.shape[0] != block_table.shape[0] or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
+        raise ValueError(f"q must be [{block_table.shape[0]}, a multiple of {Hkv}, {D}], not {tuple(q.shape)}")
+    if q.device != k_cache.device:
+        raise ValueError("q must be on the cache's device")
+    B, Hq, _ = q.shape
+    ctx_lens = _int32_vector(ctx_lens, B, "ctx_lens", q.device)
+    scale = scale if scale is not None else 1.0 / math.sqrt(D)
+    if not q.is_cuda:
+        return _decode_attention_int8_cpu(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale)
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"q must be bf16 on a GPU, not {q.dtype}")
+    if D not in (64, 128, 256):
+        raise ValueError(f"head_dim must be 64, 128 or 256 on a GPU, not {D}")
+    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty_like(q)
+    table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    for b0 in range(0, B, 8192):                       # the kernel keeps a running count per sequence in shared memory
+        n = min(8192, B - b0)
+        with torch.cuda.device(q.device):
+            size = N.cuda().ax_decode_int8_workspace(n, Hq, Hkv, D, table.shape[1], P)
+        ws = torch.empty(size, dtype=torch.float32, device=q.device)
+        N.launch("ax_decode_int8", q.device, q[b0:].data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(), v_amax.data_ptr(),
+                 table[b0:].data_ptr(), ctx_lens[b0:].data_ptr(), out[b0:].data_ptr(), n, Hq, Hkv, D, P, table.shape[1], pages, scale,
+                 ws.data_ptr(), N.status_ptr(q.device))
+    return out
+
+
+def _decode_attention_int8_cpu(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale):
+    B, Hq, D = q.shape
+    Hkv, P = k_cache.shape[1], k_cache.shape[2]
+    out = torch.zeros((B, Hq, D), dtype=torch.float32)
+    for b, n in enumerate(ctx_lens.tolist()):
+        if n == 0:
+            continue
+        if not 0 < n <= block_table.shape[1] * P:
+            raise ValueError(f"sequence {b}: context {n} does not fit its table")
+        pg = block_table[b, :(n + P - 1) // P].long()
+        if int(pg.min()) < 0 or int(pg.max()) >= k_cache.shape[0]:
+            raise ValueError(f"sequence {b}: the block table names a page outside the cache")
+        kk = (k_cache[pg].float() * (k_amax[pg] / 127.0)[:, :, None, None]).transpose(0, 1).reshape(Hkv, -1, D)[:, :n]
+        vv = (v_cache[pg].float() * (v_amax[pg] / 127.0)[:, :, None, None, None]).permute(1, 0, 2, 4, 3).reshape(Hkv, -1, D)[:, :n]
+        s = torch.einsum("hgd,hnd->hgn", q[b].float().view(Hkv, -1, D), kk) * scale
+        out[b] = torch.einsum("hgn,hnd->hgd", torch.softmax(s, -1), vv).reshape(Hq, D)
+    return out.to(q.dtype)

@@ -1,0 +1,192 @@
+"""int8 paged cache on the GPU: writes and decode attention against the definition in 64 bits."""
+import pytest
+import torch
+
+import _int8 as R
+from axonml_b200.ops import paged
+
+pytestmark = pytest.mark.gpu
+
+
+def _table(need, extra=2, seed=0):
+    g = torch.Generator().manual_seed(seed)
+    perm = torch.randperm(sum(need) + extra, generator=g).tolist()
+    table, at = torch.zeros(len(need), max(need + [1]), dtype=torch.int32), 0
+    for b, c in enumerate(need):
+        table[b, :c] = torch.tensor(perm[at:at + c], dtype=torch.int32)
+        at += c
+    return table, sum(need) + extra
+
+
+@pytest.mark.parametrize("lens,starts", [([1], [0]), ([1] * 5, [0, 15, 16, 33, 7]), ([40, 0, 3, 17], [0, 5, 30, 31]), ([300, 1, 77], [9, 0, 64]),
+                                         ([1] * 70, [i * 3 for i in range(70)])])
+@pytest.mark.parametrize("Hkv,P,D", [(1, 16, 64), (3, 32, 128), (2, 64, 256), (8, 16, 128), (2, 16, 80)])
+def test_write(lens, starts, Hkv, P, D, kernel_status):
+    table, pages = _table([(s + n + P - 1) // P for s, n in zip(starts, lens)])
+    T = sum(lens)
+    k, v = torch.randn(T + 3, Hkv, D, device="cuda").bfloat16(), (torch.randn(T + 3, Hkv, D, device="cuda") * 3).bfloat16()
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    kc, vc, ka, va = R.make_cache(pages, Hkv, P, D, "cuda")
+    want_k = R.write(kc.double(), ka.double(), k, table.tolist(), starts, cu.tolist())
+    want_v = R.write(R.v_rows(vc).double(), va.double(), v, table.tolist(), starts, cu.tolist())
+    st = torch.tensor(starts, dtype=torch.int32).cuda()
+    for _ in range(2):                                    # rows behind the last sequence are ignored; again changes nothing
+        paged.kv_write_int8(k, v, kc, vc, ka, va, table.cuda(), st, cu.cuda())
+        assert torch.equal(ka.double(), want_k[1]) and torch.equal(kc.double(), want_k[0])
+        assert torch.equal(va.double(), want_v[1]) and torch.equal(R.v_rows(vc).double(), want_v[0])
+
+
+def test_write_without_offsets_strided_fp32_and_zeros(kernel_status):
+    Hkv, P, D, B = 2, 16, 64, 4
+    table, pages = _table([3] * B)
+    qkv = torch.randn(B * 6, 2 * Hkv + 5, D, device="cuda")
+    qkv[:6] = 0.0                                         # a sequence of zeros
+    for dt in (torch.float32, torch.bfloat16):
+        x = qkv.to(dt)
+        k, v = x[:, 5:5 + Hkv], x[:, 5 + Hkv:]            # slices of a fused projection
+        caches = R.make_cache(pages, Hkv, P, D, "cuda", seed=1)
+        cpu = [t.cpu() for t in caches]
+        st = torch.tensor([0, 3, 30, 14], dtype=torch.int32)
+        paged.kv_write_int8(k, v, *caches, table.cuda(), st.cuda())
+        paged.kv_write_int8(k.cpu(), v.cpu(), *cpu, table, st)
+        for a, b in zip(caches, cpu):
+            assert torch.equal(a.cpu(), b)
+
+
+def test_write_reports_what_does_not_fit():
+    """Bad rows are skipped and reported; the others are written."""
+    from axonml_b200 import _native as N
+    Hkv, P, D = 2, 16, 64
+    k = torch.randn(3, Hkv, D, device="cuda").bfloat16()
+    for bad_start, bad_page in ((-1, 0), (16, 0), (0, 99), (0, -1)):
+        kc, vc, ka, va = R.make_cache(4, Hkv, P, D, "cuda")
+        before = [t.clone() for t in (kc, vc, ka, va)]
+        table = torch.tensor([[1], [bad_page], [2]], dtype=torch.int32, device="cuda")
+        st = torch.tensor([0, bad_start, 0], dtype=torch.int32, device="cuda")
+        paged.kv_write_int8(k, k, kc, vc, ka, va, table, st)
+        with pytest.raises(N.KernelTimeout):
+            N.check_status()
+        for t, o in zip((kc, vc, ka, va), before):
+            assert torch.equal(t[0], o[0]) and torch.equal(t[3], o[3])
+        assert ka[1].eq(k[0].float().abs().amax(-1)).all() and ka[2].eq(k[2].float().abs().amax(-1)).all()
+
+
+def _attend(B, Hkv, G, D, P, ctx, seed=0, spare=0):
+    table, pages = _table([(n + P - 1) // P for n in ctx], seed=seed)
+    if spare:
+        table = torch.cat([table, torch.full((B, spare), -7, dtype=torch.int32)], 1)      # entries past a context are not read
+    kc, vc, ka, va = R.make_cache(pages, Hkv, P, D, "cuda", seed=seed)
+    q = torch.randn(B, Hkv * G, D, device="cuda").bfloat16()
+    cl = torch.tensor(ctx, dtype=torch.int32).cuda()
+    got = paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl)
+    want, off = R.attention(q, kc, R.v_rows(vc), ka, va, table.tolist(), ctx, R.default_scale(D))
+    assert got.dtype == torch.bfloat16
+    assert ((got.double() - want).abs() <= off + torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + off)).all()
+    return got
+
+
+@pytest.mark.parametrize("Hkv,G,D,P", [(8, 4, 128, 16), (1, 1, 64, 16), (2, 8, 128, 32), (3, 5, 64, 64), (2, 16, 128, 16), (1, 37, 128, 16),
+                                       (2, 2, 256, 16), (1, 12, 256, 32), (4, 7, 64, 16), (16, 1, 128, 16)])
+@pytest.mark.parametrize("ctx", [[1], [16], [17], [777], [0], [0, 5, 0, 0, 300, 64, 0], [2000, 3, 1000]])
+def test_attention(Hkv, G, D, P, ctx, kernel_status):
+    got = _attend(len(ctx), Hkv, G, D, P, ctx, spare=2)
+    for b, n in enumerate(ctx):
+        if n == 0:
+            assert got[b].eq(0).all()
+
+
+def test_attention_many_sequences_and_a_long_one(kernel_status):
+    g = torch.Generator().manual_seed(3)
+    _attend(300, 2, 4, 128, 16, [int(x) for x in torch.randint(0, 90, (300,), generator=g)], seed=3)
+    _attend(2, 1, 8, 64, 16, [60000, 11], seed=4)
+    _attend(40, 8, 4, 128, 16, [int(x) for x in torch.randint(1, 2500, (40,), generator=g)], seed=5)
+
+
+def test_attention_extreme_scores_and_scales(kernel_status):
+    """One token that takes all the weight, q rows of very different sizes, a zero q, pages of zero magnitude."""
+    Hkv, G, D, P, n = 2, 4, 128, 16, 200
+    table, pages = _table([(n + P - 1) // P])
+    kc, vc, ka, va = R.make_cache(pages, Hkv, P, D, "cuda", seed=9)
+    q = torch.randn(1, Hkv * G, D, device="cuda").bfloat16()
+    q[0, 0] *= 1e4
+    q[0, 1] *= 1e-6
+    q[0, 2] = 0
+    q[0, 3, ::2] *= 1e-5
+    ka[table[0, 3]] = 0.0
+    va[table[0, 4]] = 0.0
+    va[table[0, 5]] *= 1000
+    cl = torch.tensor([n], dtype=torch.int32).cuda()
+    for scale in (None, 0.5, 1e-4):
+        got = paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl, scale)
+        want, off = R.attention(q, kc, R.v_rows(vc), ka, va, table.tolist(), [n], R.default_scale(D) if scale is None else scale)
+        assert ((got.double() - want).abs() <= off + torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + off)).all()
+    # a page that is not finite reaches its own sequence and head only
+    ka[table[0, 0], 1] = float("nan")
+    got = paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl)
+    assert got[0, :G].isfinite().all() and got[0, G:].isnan().any()
+    # and not where it lies behind the context
+    cl16 = torch.tensor([16], dtype=torch.int32).cuda()
+    ka[table[0, 0], 1] = 1.0
+    va[table[0, 1]] = float("inf")
+    assert paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl16).isfinite().all()
+
+
+def test_attention_reports_bad_pages_and_contexts():
+    from axonml_b200 import _native as N
+    kc, vc, ka, va = R.make_cache(4, 2, 16, 64, "cuda")
+    q = torch.randn(3, 4, 64, device="cuda").bfloat16()
+    cl = torch.tensor([20, 30, 9], dtype=torch.int32).cuda()
+    for table, ctx in (([[0, 1], [2, 99], [3, 0]], cl), ([[0, 1], [-1, 2], [3, 0]], cl), ([[0, 1], [2, 1], [3, 0]], cl + torch.tensor([0, 90, 0]).cuda().int())):
+        t = torch.tensor(table, dtype=torch.int32)
+        got = paged.decode_attention_int8(q, kc, vc, ka, va, t.cuda(), ctx)
+        with pytest.raises(N.KernelTimeout):
+            N.check_status()
+        for b in (0, 2):
+            want, off = R.attention(q[b:b + 1], kc, R.v_rows(vc), ka, va, table[b:b + 1], [int(cl[b])], R.default_scale(64))
+            assert ((got[b:b + 1].double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
+
+
+@pytest.mark.parametrize("D,dt,err", [(96, torch.bfloat16, ValueError), (64, torch.float32, TypeError)])
+def test_attention_gpu_refusals(D, dt, err):
+    c = R.make_cache(2, 1, 16, D, "cuda")
+    with pytest.raises(err):
+        paged.decode_attention_int8(torch.zeros(1, 1, D, device="cuda", dtype=dt), *c, torch.zeros(1, 1, dtype=torch.int32, device="cuda"),
+                                    torch.ones(1, dtype=torch.int32, device="cuda"))
+
+
+def test_write_then_attend_in_a_graph_and_on_another_stream(kernel_status):
+    """Decode steps captured once and replayed: the write feeds the attention; two graphs share one cache in turn."""
+    Hkv, G, D, P, B = 2, 4, 128, 16, 3
+    table, pages = _table([4] * B)
+    caches, eager = R.make_cache(pages, Hkv, P, D, "cuda", zero=True), R.make_cache(pages, Hkv, P, D, "cuda", zero=True)
+    tab = table.cuda()
+    x = torch.zeros(2, B, Hkv, D, device="cuda").bfloat16()
+    q = torch.zeros(B, Hkv * G, D, device="cuda").bfloat16()
+    pos = torch.zeros(B, dtype=torch.int32, device="cuda")
+
+    def step(c):
+        paged.kv_write_int8(x[0], x[1], *c, tab, pos)
+        return paged.decode_attention_int8(q, *c, tab, pos + 1)
+    step([t.clone() for t in caches])
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = step(caches)
+        graphs.append((g, out))
+    for t in caches:
+        t.zero_()
+    side = torch.cuda.Stream()
+    for n in range(40):
+        x.copy_(torch.randn(2, B, Hkv, D))
+        q.copy_(torch.randn(B, Hkv * G, D))
+        pos.fill_(n)
+        g, out = graphs[n % 2]
+        g.replay()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            want = step(eager)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(out, want)
+    for a, b in zip(caches, eager):
+        assert torch.equal(a, b)
