@@ -22,25 +22,6 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 v) { return __bfloat162float
 __device__ __forceinline__ void from_f(float v, float* p) { *p = v; }
 __device__ __forceinline__ void from_f(float v, __nv_bfloat16* p) { *p = __float2bfloat16_rn(v); }
 
-// Eight consecutive values.
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  uint4 u;
-  u.x = pack_bf16x2(v[0], v[1]); u.y = pack_bf16x2(v[2], v[3]); u.z = pack_bf16x2(v[4], v[5]); u.w = pack_bf16x2(v[6], v[7]);
-  *reinterpret_cast<uint4*>(p) = u;
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
 __device__ __forceinline__ float round_to(float v, const float*) { return v; }
 __device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
@@ -55,43 +36,6 @@ struct RowArgs {
   int D;
   float eps;
 };
-
-// One value of element c of the row, the product t (norm), the gated value (SwiGLU) or x itself.
-// `sq` gets the square that the norm sums.
-template <int MODE, typename T, typename WT>
-__device__ __forceinline__ float one_value(const RowArgs& a, const T* x, const T* r, T* h, int c, bool write_h, float& sq) {
-  float v = to_f(x[c]);
-  if (MODE == kSwiglu) return siluf_(v) * to_f(x[a.D + c]);
-  if (MODE == kPlain) return v;
-  if (r != nullptr) {
-    v = round_to(v + to_f(r[c]), h);
-    if (write_h) from_f(v, h + c);
-  }
-  sq = v * v;
-  return __fmul_rn(v, to_f(((const WT*)a.w)[c]));
-}
-template <int MODE, typename T, typename WT>
-__device__ __forceinline__ void eight_values(const RowArgs& a, const T* x, const T* r, T* h, int c, bool write_h, float (&t)[8], float& sq) {
-  load8(x + c, t);
-  if (MODE == kSwiglu) {
-    float u[8];
-    load8(x + a.D + c, u);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) t[j] = siluf_(t[j]) * u[j];
-  } else if (MODE == kNorm) {
-    if (r != nullptr) {
-      float rv[8];
-      load8(r + c, rv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) t[j] = round_to(t[j] + rv[j], h);
-      if (write_h) store8(h + c, t);
-    }
-    float wv[8];
-    load8((const WT*)a.w + c, wv);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) { sq += t[j] * t[j]; t[j] = __fmul_rn(t[j], wv[j]); }
-  }
-}
 
 // Sum and largest bits over the block; every thread gets both.
 __device__ __forceinline__ void block_stats(float& sum, uint32_t& top) {
@@ -109,101 +53,158 @@ __device__ __forceinline__ void block_stats(float& sum, uint32_t& top) {
 
 // KEEP: VPT groups of eight values stay in registers (D <= VPT * 8 * threads).  Otherwise the row
 // is walked twice.  VEC: rows and D allow 16-byte accesses; otherwise a thread's values lie
-// blockDim apart, so that a warp's accesses are still contiguous.
+// blockDim apart, so that a warp's accesses are still contiguous.  All loads of a walk come before its
+// stores of h: the compiler may not move a load across a store that could alias it.
 template <int MODE, typename T, typename WT, int VPT, bool KEEP, bool VEC>
-__global__ void __launch_bounds__(1024) int8_rows_kernel(const RowArgs a) {
+__global__ void __launch_bounds__(VPT == 4 ? 512 : 1024) int8_rows_kernel(const RowArgs a) {
   const long row = blockIdx.x;
   const T* x = (const T*)a.x + row * a.xs;
-  const T* r = (MODE == kNorm && a.res != nullptr) ? (const T*)a.res + row * a.rs : nullptr;
-  T* h = (MODE == kNorm && a.res != nullptr) ? (T*)a.h + row * a.hs : nullptr;
+  const bool res = MODE == kNorm && a.res != nullptr;
+  const T* r = res ? (const T*)a.res + row * a.rs : nullptr;
+  T* h = res ? (T*)a.h + row * a.hs : nullptr;
+  const WT* w = (const WT*)a.w;
   int8_t* q = a.q + row * a.qs;
   const int tid = threadIdx.x, n = blockDim.x;
-  float t[KEEP ? VPT : 1][8];
-  float sum = 0.f;
-  uint32_t top = 0;
-  if (VEC) {
-    const int steps = KEEP ? VPT : (a.D + 8 * n - 1) / (8 * n);
+  constexpr int W = VEC ? 8 : 1;                 // values of an access
+  constexpr int S = VEC ? VPT : VPT * 8;         // accesses of a thread (KEEP)
+  float t[VPT][8];
+  float sum = 0.f, most = 0.f;
+
+  // values of accesses [i0, i0 + S) of this thread into t; `out` says whether h is written
+  auto walk = [&](int i0, bool out) {
+    if constexpr (VEC) {
+      Raw8<T> xv[VPT], second[MODE == kPlain ? 1 : VPT];
 #pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int c = (i * n + tid) * 8;
-      if (c < a.D) {
-        float (&v)[8] = t[KEEP ? i : 0];
-        eight_values<MODE, T, WT>(a, x, r, h, c, true, v, sum);
+      for (int i = 0; i < VPT; ++i) {
+        const int c = ((i0 + i) * n + tid) * 8;
+        if (c < a.D) {
+          xv[i].load(x + c);
+          if (MODE == kSwiglu) second[i].load(x + a.D + c);
+          if (MODE == kNorm && res) second[i].load(r + c);
+        }
+      }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
+      for (int i = 0; i < VPT; ++i) {
+        const int c = ((i0 + i) * n + tid) * 8;
+        if (c < a.D) {
+          xv[i].get(t[i]);
+          if (MODE == kSwiglu) {
+            float u[8];
+            second[i].get(u);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[i][j] = siluf_(t[i][j]) * u[j];
+          }
+          if (MODE == kNorm) {
+            Raw8<WT> wr;
+            wr.load(w + c);
+            if (res) {
+              float u[8];
+              second[i].get(u);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) t[i][j] += u[j];
+              xv[i].set(t[i]);
+              if (out) xv[i].store(h + c);
+            }
+            float wv[8];
+            wr.get(wv);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              sum += t[i][j] * t[i][j];
+              t[i][j] = __fmul_rn(t[i][j], wv[j]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) t[i][j] = 0.f;
+        }
+      }
+    } else {
+      float second[MODE == kPlain ? 1 : VPT * 8], wv[MODE == kNorm ? VPT * 8 : 1];
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const int c = (i0 + i) * n + tid;
+        const bool in = c < a.D;
+        t[i / 8][i % 8] = in ? to_f(x[c]) : 0.f;
+        if (MODE == kSwiglu) second[i] = in ? to_f(x[a.D + c]) : 0.f;
+        if (MODE == kNorm) {
+          second[i] = in && res ? to_f(r[c]) : 0.f;
+          wv[i] = in ? to_f(w[c]) : 0.f;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < S; ++i) {
+        const int c = (i0 + i) * n + tid;
+        float& v = t[i / 8][i % 8];
+        if (MODE == kSwiglu) v = siluf_(v) * second[i];
+        if (MODE == kNorm) {
+          if (res) {
+            v = round_to(v + second[i], h);
+            if (out && c < a.D) from_f(v, h + c);
+          }
+          sum += v * v;
+          v = __fmul_rn(v, wv[i]);
+        }
       }
     }
-  } else {
-    const int steps = KEEP ? VPT * 8 : (a.D + n - 1) / n;
+  };
+  const int rounds = KEEP ? 1 : (a.D + W * S * n - 1) / (W * S * n);
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    walk(k * S, true);
 #pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int c = i * n + tid;
-      if (c < a.D) {
-        float sq = 0.f;
-        float& v = t[KEEP ? i / 8 : 0][KEEP ? i % 8 : 0];
-        v = one_value<MODE, T, WT>(a, x, r, h, c, true, sq);
-        sum += sq;
-        top = max(top, abs_bits(v));
-      }
-    }
+    for (int i = 0; i < VPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = amax_nan(most, t[i][j]);
   }
+  uint32_t top = abs_bits(most);
   block_stats(sum, top);
-  if (top < kTinyBits) top = 0;
-  const float amax = __uint_as_float(top);
-  const float inv = top ? __fdiv_rn(127.f, amax) : 0.f;
+  const Int8Grid grid = int8_grid(top);
   if (tid == 0) {
     const float rstd = MODE == kNorm ? __frsqrt_rn(__fdiv_rn(sum, (float)a.D) + a.eps) : 1.f;
+    const float amax = top < 0x00800000u ? 0.f : grid.amax;
     a.scale[row] = __fdiv_rn(__fmul_rn(amax, rstd), 127.f);
   }
-  if (VEC) {
-    const int steps = KEEP ? VPT : (a.D + 8 * n - 1) / (8 * n);
+#pragma unroll 1
+  for (int k = 0; k < rounds; ++k) {
+    // the second walk reads x and r again, not h: they round to the same sum
+    if (!KEEP) walk(k * S, false);
+    if constexpr (VEC) {
 #pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int c = (i * n + tid) * 8;
-      if (c < a.D) {
-        float (&v)[8] = t[KEEP ? i : 0];
-        // the second walk reads the inputs again, not h: with r, x + r rounds to the same h
-        if (!KEEP) eight_values<MODE, T, WT>(a, x, r, h, c, false, v, sum);
-        int s[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s[j] = top ? int8_step(v[j], amax, inv) : 0;
-        *reinterpret_cast<uint2*>(q + c) = make_uint2(pack_int8x4(s[0], s[1], s[2], s[3]), pack_int8x4(s[4], s[5], s[6], s[7]));
+      for (int i = 0; i < VPT; ++i) {
+        const int c = ((k * S + i) * n + tid) * 8;
+        uint32_t b[2];
+        int8_steps<8>(t[i], grid, b);
+        if (c < a.D) *reinterpret_cast<uint2*>(q + c) = make_uint2(b[0], b[1]);
       }
-    }
-  } else {
-    const int steps = KEEP ? VPT * 8 : (a.D + n - 1) / n;
+    } else {
 #pragma unroll
-    for (int i = 0; i < steps; ++i) {
-      const int c = i * n + tid;
-      if (c < a.D) {
-        float& v = t[KEEP ? i / 8 : 0][KEEP ? i % 8 : 0];
-        float sq;
-        if (!KEEP) v = one_value<MODE, T, WT>(a, x, r, h, c, false, sq);
-        q[c] = (int8_t)(top ? int8_step(v, amax, inv) : 0);
+      for (int i = 0; i < VPT; ++i) {
+        uint32_t b[2];
+        int8_steps<8>(t[i], grid, b);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int c = (k * S + i * 8 + j) * n + tid;
+          if (c < a.D) q[c] = (int8_t)(b[j / 4] >> (8 * (j % 4)));
+        }
       }
     }
   }
 }
 
-// Threads and groups per thread: the fewest groups that 1024 threads cover for few rows (latency:
-// all loads of the row are in flight at once), two or more groups a thread for many rows (fewer
-// warps wait at the reduction).
+// Threads and groups per thread: one group each for few rows (latency: all loads of the row are in flight
+// at once), four for many rows (a warp's share of the reduction and of the row's divisions is paid once per
+// 1024 values: 508 instructions a warp at two groups, of which 150 do not depend on them); rows up to 16384
+// wide stay in registers.
 template <int MODE, typename T, typename WT, bool VEC>
 int launch(const RowArgs& a, int rows, cudaStream_t stream) {
   const int groups = (a.D + 7) / 8;
-  int vpt = 1;
-  if (rows > 2 * axh::sm_count() && groups > 64) vpt = groups > 1024 ? 4 : 2;
-  while (vpt < 4 && (long)vpt * 1024 < groups) vpt *= 2;
-  int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
-  if (threads > 1024) {
-    int8_rows_kernel<MODE, T, WT, 1, false, VEC><<<rows, 1024, 0, stream>>>(a);
-  } else if (vpt == 1) {
-    int8_rows_kernel<MODE, T, WT, 1, true, VEC><<<rows, threads, 0, stream>>>(a);
-  } else if (vpt == 2) {
-    int8_rows_kernel<MODE, T, WT, 2, true, VEC><<<rows, threads, 0, stream>>>(a);
-  } else {
-    int8_rows_kernel<MODE, T, WT, 4, true, VEC><<<rows, threads, 0, stream>>>(a);
-  }
+  int vpt = groups > 1024 ? 2 : 1;   // (the scalar path stops at two: its values are 8 x as many accesses)
+  if (rows > 2 * axh::sm_count() && groups > 64) vpt = VEC && groups >= 256 ? 4 : 2;
+  const int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
+  if (threads > (vpt == 4 ? 512 : 1024)) int8_rows_kernel<MODE, T, WT, 1, false, VEC><<<rows, 1024, 0, stream>>>(a);
+  else if (vpt == 1) int8_rows_kernel<MODE, T, WT, 1, true, VEC><<<rows, threads, 0, stream>>>(a);
+  else if (vpt == 2) int8_rows_kernel<MODE, T, WT, 2, true, VEC><<<rows, threads, 0, stream>>>(a);
+  else if constexpr (VEC) int8_rows_kernel<MODE, T, WT, 4, true, VEC><<<rows, threads, 0, stream>>>(a);
   return (int)cudaGetLastError();
 }
 

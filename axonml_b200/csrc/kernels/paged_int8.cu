@@ -86,109 +86,158 @@ __device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& 
   return false;
 }
 
-__device__ __forceinline__ float elem(const float* p) { return *p; }
-__device__ __forceinline__ float elem(const __nv_bfloat16* p) { return __bfloat162float(*p); }
-__device__ __forceinline__ void load8(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 u = *reinterpret_cast<const uint4*>(p);
-  const float2 a = unpack_bf16x2(u.x), b = unpack_bf16x2(u.y), c = unpack_bf16x2(u.z), d = unpack_bf16x2(u.w);
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y; v[4] = c.x; v[5] = c.y; v[6] = d.x; v[7] = d.y;
-}
-__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-}
-
-// rint(q a_old / a_new); the same border rule as int8_step
-__device__ __forceinline__ int rescale_step(int q, float old, float grown, float ratio) {
-  const float f = (float)q * ratio;
-  float n = rintf(f);
-  if (!(fabsf(fabsf(f - n) - 0.5f) >= 1e-4f)) n = rintf(__fdiv_rn(__fmul_rn((float)q, old), grown));
-  return __float2int_rn(n);
-}
+// rint(q a_old / a_new) of four bytes; the same border rule as int8_steps
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, float grown, float ratio) {
-  return pack_int8x4(rescale_step((int8_t)(w & 255), old, grown, ratio), rescale_step((int8_t)((w >> 8) & 255), old, grown, ratio),
-                     rescale_step((int8_t)((w >> 16) & 255), old, grown, ratio), rescale_step((int8_t)(w >> 24), old, grown, ratio));
+  uint32_t b[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float q = (float)(int8_t)((w >> (8 * j)) & 255u), f = q * ratio;
+    float r = __fadd_rn(f, kRound);
+    if (fabsf(f - __fadd_rn(r, -kRound)) > kBorder) r = __fadd_rn(__fdiv_rn(__fmul_rn(q, old), grown), kRound);
+    b[j] = __float_as_uint(r);
+  }
+  return pack_low_bytes(b[0], b[1], b[2], b[3]);
 }
 
-// Grid (pieces, Hkv, 2): one block per page piece and head of K (z = 0) or V (z = 1).  The new rows are
-// read twice, the second time from L1: once for the magnitude, once to be rounded.
+// 0xff in byte j of word w where lo <= 4 w + j < hi
+__device__ __forceinline__ uint32_t byte_mask(int w, int lo, int hi) {
+  const int a = min(max(lo - 4 * w, 0), 4), b = min(max(hi - 4 * w, 0), 4);
+  const uint32_t below_b = b == 4 ? 0xffffffffu : (1u << (8 * b)) - 1u, below_a = a == 4 ? 0xffffffffu : (1u << (8 * a)) - 1u;
+  return below_b & ~below_a;
+}
+
+constexpr int kHalf = 64;     // threads of a block that work on K, and as many on V
+
+// Grid (pieces, Hkv): one block per page piece and head; half of its threads take K, half V.  The new
+// rows are read twice, the second time from L1: once for the magnitude, once to be rounded.
+// K: a thread rounds eight dims of a token.  V: four lanes take eight dims of sixteen slots, four slots each
+// (16-byte loads of four tokens), and exchange words so that each lane stores two dims' sixteen slots whole.
 template <typename T>
-__global__ void __launch_bounds__(128) kv_write_int8_kernel(const WriteArgs a) {
-  __shared__ uint32_t s_top[4];
+__global__ void __launch_bounds__(2 * kHalf) kv_write_int8_kernel(const WriteArgs a) {
+  __shared__ uint32_t s_top[2 * kHalf / 32];
   Piece pc;
   if (!find_piece(a, (int)blockIdx.x, pc)) return;           // uniform over the block
-  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool is_v = blockIdx.z != 0;
+  const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const bool is_v = threadIdx.x >= kHalf;
+  const int tid = threadIdx.x & (kHalf - 1);
   const long ts = is_v ? a.v_ts : a.k_ts;
   const T* x = (const T*)(is_v ? a.v : a.k) + (long)pc.src * ts + (long)h * (is_v ? a.v_hs : a.k_hs);
   const long group = (long)pc.page * a.Hkv + h;
   float* amax_p = (is_v ? a.va : a.ka) + group;
   int8_t* dst = (is_v ? a.vc : a.kc) + group * a.P * a.D;
-
-  uint32_t top = 0;
-  const int per_row = a.D / 8;
-  for (int i = tid; i < pc.count * per_row; i += 128) {
-    const int t = i / per_row, c = (i - t * per_row) * 8;
-    float v[8];
-    load8(x + t * ts + c, v);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) top = max(top, abs_bits(v[j]));
-  }
   const float before = pc.first > 0 ? *amax_p : 0.f;
-  top = __reduce_max_sync(0xffffffffu, top);
+
+  float most = 0.f;
+  const int per_row = a.D / 8, end = pc.first + pc.count;
+  // Both halves walk the rows as they lie; V's lanes come back to them in another order.
+#pragma unroll 4
+  for (int i = tid; i < pc.count * per_row; i += kHalf) {
+    const int t = i / per_row, c = (i - t * per_row) * 8;
+    Raw8<T> raw;
+    raw.load(x + t * ts + c);
+    float v[8];
+    raw.get(v);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = amax_nan(most, v[j]);
+  }
+  uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most));
   if (lane == 0) s_top[warp] = top;
   __syncthreads();                                           // also: every thread has read the old magnitude
-  top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
-  const uint32_t old_bits = abs_bits(before) < kTinyBits ? 0u : abs_bits(before);
+  const int w0 = is_v ? kHalf / 32 : 0;
+#pragma unroll
+  for (int i = 0; i < kHalf / 32; ++i) top = max(top, s_top[w0 + i]);
+  const uint32_t old_bits = abs_bits(before) < 0x00800000u ? 0u : abs_bits(before);
   top = max(top, old_bits);
-  if (top < kTinyBits) top = 0;
+  if (top < 0x00800000u) top = 0;
+  const Int8Grid grid = int8_grid(top);
   const float grown = __uint_as_float(top), old = __uint_as_float(old_bits);
-  const float inv = top ? __fdiv_rn(127.f, grown) : 0.f;
   const bool again = top > old_bits && pc.first > 0;
-  const float ratio = again ? __fdiv_rn(old, grown) : 1.f;
+  const float ratio = again && grid.live ? __fdiv_rn(old, grown) : 0.f;
   if (tid == 0) *amax_p = grown;
 
   if (!is_v) {
     if (again) {
       uint2* rows = reinterpret_cast<uint2*>(dst);
-      for (int i = tid; i < pc.first * per_row; i += 128) {
+      for (int i = tid; i < pc.first * per_row; i += kHalf) {
         const uint2 w = rows[i];
         rows[i] = make_uint2(rescale4(w.x, old, grown, ratio), rescale4(w.y, old, grown, ratio));
       }
     }
-    for (int i = tid; i < pc.count * per_row; i += 128) {
+#pragma unroll 4
+    for (int i = tid; i < pc.count * per_row; i += kHalf) {
       const int t = i / per_row, c = (i - t * per_row) * 8;
+      Raw8<T> raw;
+      raw.load(x + t * ts + c);
       float v[8];
-      load8(x + t * ts + c, v);
-      int s[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) s[j] = top ? int8_step(v[j], grown, inv) : 0;
-      *reinterpret_cast<uint2*>(dst + (long)(pc.first + t) * a.D + c) =
-          make_uint2(pack_int8x4(s[0], s[1], s[2], s[3]), pack_int8x4(s[4], s[5], s[6], s[7]));
+      raw.get(v);
+      uint32_t b[2];
+      int8_steps<8>(v, grid, b);
+      *reinterpret_cast<uint2*>(dst + (long)(pc.first + t) * a.D + c) = make_uint2(b[0], b[1]);
     }
-  } else {
-    // sixteen slots of one dim are one 16-byte word; slots that are neither old nor new keep their byte
-    const int g0 = again ? 0 : pc.first / 16, g1 = (pc.first + pc.count + 15) / 16, end = pc.first + pc.count;
-    for (int i = tid; i < (g1 - g0) * a.D; i += 128) {
-      const int g = g0 + i / a.D, d = i % a.D, s0 = g * 16;
-      uint4* p = reinterpret_cast<uint4*>(dst + (long)g * 16 * a.D + d * 16);
-      uint32_t w[4] = {0u, 0u, 0u, 0u};
-      if (s0 < pc.first || s0 + 16 > end) {
-        const uint4 o = *p;
-        w[0] = o.x; w[1] = o.y; w[2] = o.z; w[3] = o.w;
-      }
+    return;
+  }
+  const int g0 = again ? 0 : pc.first / 16, g1 = (end + 15) / 16;
+  const int i4 = tid & 3, units = (g1 - g0) * per_row;       // a unit: four lanes, sixteen slots, eight dims
+  for (int u0 = 0; u0 < units; u0 += kHalf / 4) {
+    const int u = u0 + tid / 4;
+    const bool in = u < units;
+    const int g = g0 + (in ? u / per_row : 0), c = in ? (u % per_row) * 8 : 0, s0 = g * 16;
+    uint32_t steps[4][2];                                    // [slot 4 i4 + .][dims 0-3 | 4-7]
 #pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const int slot = s0 + j;
-        int val = (int8_t)((w[j / 4] >> (8 * (j % 4))) & 255);
-        if (slot < pc.first) {
-          if (again) val = rescale_step(val, old, grown, ratio);
-        } else if (slot < end) {
-          val = top ? int8_step(elem(x + (slot - pc.first) * ts + d), grown, inv) : 0;
-        }
-        w[j / 4] = (w[j / 4] & ~(255u << (8 * (j % 4)))) | ((uint32_t)(val & 255) << (8 * (j % 4)));
+    for (int k = 0; k < 4; ++k) {
+      const int slot = s0 + 4 * i4 + k;
+      steps[k][0] = steps[k][1] = 0u;
+      if (in && slot >= pc.first && slot < end) {
+        Raw8<T> raw;
+        raw.load(x + (slot - pc.first) * ts + c);
+        float v[8];
+        raw.get(v);
+        int8_steps<8>(v, grid, steps[k]);
       }
-      *p = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    // bytes [slot][dim] -> words word[dim] of this lane's four slots
+    uint32_t word[8];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t lo01 = __byte_perm(steps[0][half], steps[1][half], 0x5140), hi01 = __byte_perm(steps[0][half], steps[1][half], 0x7362);
+      const uint32_t lo23 = __byte_perm(steps[2][half], steps[3][half], 0x5140), hi23 = __byte_perm(steps[2][half], steps[3][half], 0x7362);
+      word[4 * half] = __byte_perm(lo01, lo23, 0x5410);
+      word[4 * half + 1] = __byte_perm(lo01, lo23, 0x7632);
+      word[4 * half + 2] = __byte_perm(hi01, hi23, 0x5410);
+      word[4 * half + 3] = __byte_perm(hi01, hi23, 0x7632);
+    }
+    // four lanes hold four slots each of dims c .. c + 7; lane i4 collects dims c + i4 and c + 4 + i4 in two
+    // exchanges (with the neighbour at distance 1, then 2)
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      uint32_t* m = word + 4 * half;
+      const bool odd = i4 & 1, up = i4 & 2;
+      // distance 1: keep dims of this lane's parity
+      const uint32_t s1 = __shfl_xor_sync(0xffffffffu, odd ? m[0] : m[1], 1), s2 = __shfl_xor_sync(0xffffffffu, odd ? m[2] : m[3], 1);
+      // a[d][lane parity]: dims {i4 & 1, 2 + (i4 & 1)}, slots of lanes (even, odd) of the pair
+      const uint32_t d0e = odd ? s1 : m[0], d0o = odd ? m[1] : s1;
+      const uint32_t d2e = odd ? s2 : m[2], d2o = odd ? m[3] : s2;
+      // distance 2: lanes 0, 1 keep dims 0, 1; lanes 2, 3 keep dims 2, 3
+      const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? d0e : d2e, 2), r1 = __shfl_xor_sync(0xffffffffu, up ? d0o : d2o, 2);
+      uint32_t out[4];
+      out[0] = up ? r0 : d0e;
+      out[1] = up ? r1 : d0o;
+      out[2] = up ? d2e : r0;
+      out[3] = up ? d2o : r1;
+      if (in) {
+        uint4* p = reinterpret_cast<uint4*>(dst + (long)g * 16 * a.D + (c + 4 * half + i4) * 16);
+        if (s0 < pc.first || s0 + 16 > end) {                // slots that are neither old nor new keep their byte
+          const uint4 o = *p;
+          const uint32_t was[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint32_t fresh = byte_mask(k, pc.first - s0, end - s0), held = again ? byte_mask(k, 0, pc.first - s0) : 0u;
+            const uint32_t scaled = held ? rescale4(was[k], old, grown, ratio) : 0u;
+            out[k] = (out[k] & fresh) | (scaled & held) | (was[k] & ~(fresh | held));
+          }
+        }
+        *p = make_uint4(out[0], out[1], out[2], out[3]);
+      }
     }
   }
 }
@@ -387,8 +436,11 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
         for (int j = 0; j < NJ; ++j) {
           float x0[8], x1[8];
           if (live) {
-            load8(qp + (i4 + 4 * j) * 16, x0);
-            load8(qp + (i4 + 4 * j) * 16 + 8, x1);
+            Raw8<__nv_bfloat16> q0, q1;
+            q0.load(qp + (i4 + 4 * j) * 16);
+            q1.load(qp + (i4 + 4 * j) * 16 + 8);
+            q0.get(x0);
+            q1.get(x1);
           }
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
@@ -656,9 +708,9 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   // a row of n tokens touches at most (n - 1) / P + 2 pages; a single token one
   const long rows = B < T ? B : T;
   const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
-  const dim3 grid((unsigned)pieces, Hkv, 2);
-  if (dt == 1) kv_write_int8_kernel<__nv_bfloat16><<<grid, 128, 0, stream>>>(a);
-  else kv_write_int8_kernel<float><<<grid, 128, 0, stream>>>(a);
+  const dim3 grid((unsigned)pieces, Hkv);
+  if (dt == 1) kv_write_int8_kernel<__nv_bfloat16><<<grid, 2 * kHalf, 0, stream>>>(a);
+  else kv_write_int8_kernel<float><<<grid, 2 * kHalf, 0, stream>>>(a);
   return (int)cudaGetLastError();
 }
 
