@@ -182,29 +182,42 @@ class KernelTimeout(RuntimeError):
         self.code, self.where, self.block = code, where, block
 
 
-def launch(name: str, device: torch.device, *args) -> None:
-    """Calls entry point ``name`` of ``_SIGNATURES`` on ``device``'s current stream (its last argument),
-    also when that is not the current device, and raises on a non-zero code."""
-    fn = getattr(cuda(), name)
-    if device.index == torch._C._cuda_getDevice():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
+_ENTRIES: dict = {}
+_current_device = getattr(torch._C, "_cuda_getDevice", None)
+_current_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def launch(name: str, index: int, *args) -> None:
+    """Calls entry point ``name`` of ``_SIGNATURES`` on the current stream of GPU ``index`` (the entry's
+    last argument), also when that is not the current device, and raises on a non-zero code."""
+    fn = _ENTRIES.get(name)
+    if fn is None:
+        fn = _ENTRIES[name] = getattr(cuda()._lib, name)
+    _CUDA.launches += 1
+    if index == _current_device():
+        rc = fn(*args, _current_stream(index))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(device.index))
-    if rc != 0:
+        with torch.cuda.device(index):
+            rc = fn(*args, _current_stream(index))
+    if rc:
         raise NativeError(f"{name} failed with code {rc}")
 
 
-def status_ptr(device: torch.device) -> int:
-    """Address of ``device``'s status word.  The word has to exist before a stream capture: made inside
-    one, it would be cleared by every replay."""
-    t = _STATUS.get(("cuda", device.index))
-    if t is None:
-        if torch.cuda.is_current_stream_capturing():
+_STATUS_PTR: dict = {}
+
+
+def status_ptr(index: int) -> int:
+    """Address of the status word of GPU ``index``.  The word has to exist before a stream capture: made
+    inside one, it would be cleared by every replay."""
+    p = _STATUS_PTR.get(index)
+    if p is None:
+        dev = torch.device("cuda", index)
+        if ("cuda", index) not in _STATUS and torch.cuda.is_current_stream_capturing():
             raise NativeError("call the operator once before capturing it: its status word does not exist yet")
-        t = status_word(device)
-        torch.cuda.current_stream(device).synchronize()      # other streams use the word from now on
-    return t.data_ptr()
+        p = _STATUS_PTR[index] = status_word(dev).data_ptr()
+        if not torch.cuda.is_current_stream_capturing():
+            torch.cuda.current_stream(dev).synchronize()     # other streams use the word from now on
+    return p
 
 
 def check_status(device=None) -> None:

@@ -11,6 +11,13 @@
 
 namespace ax {
 
+// Programmatic dependent launch: a kernel launched with launch_chained may start while the one before it on
+// the stream still runs, and sets itself up (barriers, TMEM, descriptors) until chain_wait returns, which is when that
+// kernel has ended and its writes are visible.  Every thread that touches memory calls chain_wait first, in
+// every block, so that a grid never ends before the one it follows.  chain_ready lets the next grid start.
+__device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void chain_ready() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Largest magnitudes travel as the bits of |x|: integer order is the order of non-negative floats, and
 // NaN lies above infinity, so a NaN in a group reaches the group's magnitude.
 __device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
@@ -120,3 +127,25 @@ struct Raw8<float> {
 };
 
 }  // namespace ax
+
+namespace axh {
+// Launch with the attribute above, and in clusters of `cluster` blocks along x where that is more than one.
+template <typename... P, typename... A>
+int launch_chained(void (*kern)(P...), dim3 grid, dim3 block, int smem, int cluster, cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return (int)cudaLaunchKernelEx(&cfg, kern, args...);
+}
+}  // namespace axh

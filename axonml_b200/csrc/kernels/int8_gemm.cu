@@ -41,7 +41,7 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t d, uint64_t a, uint64_t b,
 }
 __device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
   uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
@@ -60,14 +60,17 @@ struct GemmArgs {
 
 // ------------------------------------------------------------------------------ few rows
 // Grid (S * ceil(N / 128), ceil(M / BN)), clusters of S along x: rank r of a cluster takes its share of
-// the k blocks of one 128-channel tile.  Warp 0 loads, warp 1 multiplies, all four read TMEM.
+// the k blocks of one tile of 128 channels and BN tokens.  Warp 0 loads, warp 1 multiplies, all four read
+// TMEM.  (256 channels a block, which halve how often the tokens are read, were 0 to 10 % slower at every size tried.)
 template <int BN>
 struct StreamCfg {
   static constexpr int kStageA = kRowsA * kBytesK, kStageB = BN * kBytesK, kStage = kStageA + kStageB;
-  static constexpr int kStages = BN <= 32 ? 5 : (BN == 64 ? 4 : 6);
+  // half of an SM's shared memory: two blocks share it, and where the tiles do not fill the device evenly
+  // the bandwidth still does (128 x 28672 x 4096: 27.9 us, 40.6 with one block an SM)
+  static constexpr int kStages = 102 * 1024 / kStage;
   static constexpr int kTmem = BN < 32 ? 32 : BN;
   static constexpr int kSmem = 1024 + kStages * kStage + 256;
-  static_assert(BN * kRowsA * 4 <= kStages * kStage, "the reduction buffer lies over the stages");
+  static_assert(BN * kRowsA * 4 <= kStages * kStage, "the exchange buffer lies over the stages");
 };
 
 template <int BN, typename OutT>
@@ -100,6 +103,8 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  chain_ready();
+  chain_wait();
 
   if (warp == 0) {
     if (lane == 0) {
@@ -149,13 +154,13 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (ok) {
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(t_row + c, r);
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(t_row + c, v);
         tc_wait_ld();
 #pragma unroll
         for (int j = 0; j < 16; ++j)
           if (c + j < cols && n < p.N)
-            store_out(out + (long)(c + j) * p.ldo, __int2float_rn((int)r[j]) * p.sx[m0 + c + j] * sw + bias);
+            store_out(out + (long)(c + j) * p.ldo, __int2float_rn((int)v[j]) * __ldg(p.sx + m0 + c + j) * sw + bias);
       }
     }
   } else {
@@ -165,11 +170,11 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     if (ok) {
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
-        uint32_t r[16];
-        tmem_ld_32x32b_x16(t_row + c, r);
+        uint32_t v[16];
+        tmem_ld_32x32b_x16(t_row + c, v);
         tc_wait_ld();
 #pragma unroll
-        for (int j = 0; j < 16; ++j) red[(c + j) * kRowsA + row] = (int)r[j];
+        for (int j = 0; j < 16; ++j) red[(c + j) * kRowsA + row] = (int)v[j];
       }
     }
     __syncwarp();
@@ -178,12 +183,13 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       uint32_t peer[8];
 #pragma unroll
       for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(smem_u32(red + row), s) : 0;
+#pragma unroll 4
       for (int c = rank; c < cols; c += S) {
-        int sum = 0;
+        int part[8];
 #pragma unroll
-        for (int s = 0; s < 8; ++s)
-          if (s < S) sum += (int)ld_cluster(peer[s] + (uint32_t)(c * kRowsA * 4));
-        if (n < p.N) store_out(out + (long)c * p.ldo, __int2float_rn(sum) * p.sx[m0 + c] * sw + bias);
+        for (int s = 0; s < 8; ++s) part[s] = s < S ? (int)ld_cluster(peer[s] + (uint32_t)(c * kRowsA * 4)) : 0;
+        const int sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
+        if (n < p.N) store_out(out + (long)c * p.ldo, __int2float_rn(sum) * __ldg(p.sx + m0 + c) * sw + bias);
       }
     }
     __syncwarp();
@@ -244,6 +250,8 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   cluster_sync_all();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  chain_ready();
+  chain_wait();
 
   // groups of four row blocks sweep the columns, so that pairs at work together share tiles in L2
   auto tile_at = [&](int t, int& mb, int& nb) {
@@ -439,19 +447,8 @@ int launch_stream(const void* q, long ldq, const void* w, long ldw, const GemmAr
   if (rc) return 1000 + rc;
   rc = make_map(&mx, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, p.K, p.M, ldq, kBytesK, BN);
   if (rc) return 2000 + rc;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = S;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.gridDim = dim3(S * ((p.N + kRowsA - 1) / kRowsA), (p.M + BN - 1) / BN, 1);
-  cfg.blockDim = dim3(128, 1, 1);
-  cfg.dynamicSmemBytes = C::kSmem;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, kern, mw, mx, p, S);
+  const dim3 grid(S * ((p.N + kRowsA - 1) / kRowsA), (p.M + BN - 1) / BN);
+  return axh::launch_chained(kern, grid, dim3(128), C::kSmem, S, stream, mw, mx, p, S);
 }
 
 template <int BN, typename OutT>
@@ -496,8 +493,7 @@ int launch_pair(const void* q, long ldq, const void* w, long ldw, const GemmArgs
   }
   const long tiles = (long)((p.M + 2 * kRowsA - 1) / (2 * kRowsA)) * ((p.N + BN - 1) / BN);
   const int pairs = tiles < max_pairs[dev] ? (int)tiles : max_pairs[dev];
-  cfg.gridDim = dim3(2 * pairs, 1, 1);
-  return (int)cudaLaunchKernelEx(&cfg, kern, mx, mw, mo, p);
+  return axh::launch_chained(kern, dim3(2 * pairs), dim3(kThreads), C::kSmem, 2, stream, mx, mw, mo, p);
 }
 
 template <typename OutT>

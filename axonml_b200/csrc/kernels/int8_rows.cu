@@ -69,6 +69,8 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024) int8_rows_kernel(const 
   constexpr int S = VEC ? VPT : VPT * 8;         // accesses of a thread (KEEP)
   float t[VPT][8];
   float sum = 0.f, most = 0.f;
+  chain_ready();
+  chain_wait();
 
   // values of accesses [i0, i0 + S) of this thread into t; `out` says whether h is written
   auto walk = [&](int i0, bool out) {
@@ -201,11 +203,11 @@ int launch(const RowArgs& a, int rows, cudaStream_t stream) {
   int vpt = groups > 1024 ? 2 : 1;   // (the scalar path stops at two: its values are 8 x as many accesses)
   if (rows > 2 * axh::sm_count() && groups > 64) vpt = VEC && groups >= 256 ? 4 : 2;
   const int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
-  if (threads > (vpt == 4 ? 512 : 1024)) int8_rows_kernel<MODE, T, WT, 1, false, VEC><<<rows, 1024, 0, stream>>>(a);
-  else if (vpt == 1) int8_rows_kernel<MODE, T, WT, 1, true, VEC><<<rows, threads, 0, stream>>>(a);
-  else if (vpt == 2) int8_rows_kernel<MODE, T, WT, 2, true, VEC><<<rows, threads, 0, stream>>>(a);
-  else if constexpr (VEC) int8_rows_kernel<MODE, T, WT, 4, true, VEC><<<rows, threads, 0, stream>>>(a);
-  return (int)cudaGetLastError();
+  if (threads > (vpt == 4 ? 512 : 1024)) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 1, false, VEC>, dim3(rows), dim3(1024), 0, 1, stream, a);
+  if (vpt == 1) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 1, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
+  if (vpt == 2) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 2, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
+  if constexpr (VEC) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 4, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
+  return -1;
 }
 
 template <int MODE, typename T, typename WT>

@@ -115,6 +115,8 @@ constexpr int kHalf = 64;     // threads of a block that work on K, and as many 
 template <typename T>
 __global__ void __launch_bounds__(2 * kHalf) kv_write_int8_kernel(const WriteArgs a) {
   __shared__ uint32_t s_top[2 * kHalf / 32];
+  chain_ready();
+  chain_wait();
   Piece pc;
   if (!find_piece(a, (int)blockIdx.x, pc)) return;           // uniform over the block
   const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -322,7 +324,6 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
   constexpr int NT = D / 8;                                      // 8-dim tiles of O
   constexpr int R = HG / 8;                                      // rows of the MMA a lane owns
   extern __shared__ __align__(128) uint8_t smem[];
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");   // the merge may be set up; it waits for this grid's end
   uint64_t* bars = (uint64_t*)(smem + C::kRing);
   volatile int* dead = (volatile int*)(bars + kWarps * C::kStages);
   int* prefix = (int*)(bars + kWarps * C::kStages) + 2;          // [B + 1] tiles of the sequences before
@@ -332,6 +333,8 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
     for (int i = 0; i < kWarps * C::kStages; ++i) mbar_init(&bars[i], 1);
     mbar_fence_init();
   }
+  chain_ready();                                                 // the merge may be set up
+  chain_wait();
   if (warp == 0) {
     int sum = 0;
     for (int b0 = 0; b0 < a.B; b0 += 32) {
@@ -591,6 +594,7 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
   const int b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
   const int h = hq / a.G, hg = hq % a.G, vh = h * a.nblk + hg / HG, row = hg % HG;
   const int VH = a.Hkv * a.nblk;
+  chain_wait();
   int before = 0, total = 0, tb = 0;
   for (int b0 = 0; b0 < a.B; b0 += 32) {
     const int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
@@ -605,7 +609,6 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
     tb += __shfl_xor_sync(0xffffffffu, tb, o);
   }
   __nv_bfloat16* op = a.out + ((long)b * a.Hq + hq) * D;
-  asm volatile("griddepcontrol.wait;" ::: "memory");             // the first kernel is done, its partials are visible
   if (tb == 0) {
     if (warp == 0)
       for (int d = lane; d < D; d += 32) op[d] = __float2bfloat16(0.f);
@@ -675,20 +678,9 @@ int launch_attn(AttnArgs& a, int blocks, int merge_warps, cudaStream_t stream) {
     if (e != cudaSuccess) return (int)e;
     if (dev >= 0 && dev < 64) configured[dev] = smem;
   }
-  kern<<<blocks, kWarps * 32, smem, stream>>>(a);
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return (int)e;
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;   // the merge's own set-up runs beside the first kernel's end
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(a.B * a.Hq, 1, 1);
-  cfg.blockDim = dim3(32 * merge_warps, 1, 1);
-  cfg.dynamicSmemBytes = merge_warps * (D + 2) * 4;
-  cfg.stream = stream;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return (int)cudaLaunchKernelEx(&cfg, merge_int8_kernel<D, HG>, a);
+  int rc = axh::launch_chained(kern, dim3(blocks), dim3(kWarps * 32), smem, 1, stream, a);
+  if (rc) return rc;
+  return axh::launch_chained(merge_int8_kernel<D, HG>, dim3(a.B * a.Hq), dim3(32 * merge_warps), merge_warps * (D + 2) * 4, 1, stream, a);
 }
 
 }  // namespace
@@ -709,9 +701,8 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   const long rows = B < T ? B : T;
   const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
   const dim3 grid((unsigned)pieces, Hkv);
-  if (dt == 1) kv_write_int8_kernel<__nv_bfloat16><<<grid, 2 * kHalf, 0, stream>>>(a);
-  else kv_write_int8_kernel<float><<<grid, 2 * kHalf, 0, stream>>>(a);
-  return (int)cudaGetLastError();
+  if (dt == 1) return axh::launch_chained(kv_write_int8_kernel<__nv_bfloat16>, grid, dim3(2 * kHalf), 0, 1, stream, a);
+  return axh::launch_chained(kv_write_int8_kernel<float>, grid, dim3(2 * kHalf), 0, 1, stream, a);
 }
 
 // Workers (warps) the attention kernel runs with: what fills the device, fewer for a small cache.

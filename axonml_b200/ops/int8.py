@@ -19,8 +19,9 @@ MAX_K = 131071          # 2^14 K < 2^31: the int32 sum cannot overflow
 def _aligned_rows(rows: int, cols: int, device) -> torch.Tensor:
     """int8 ``[rows, cols]`` whose rows start on 16-byte boundaries (the product's loads need that)."""
     pad = -cols % 16
-    t = torch.empty((rows, cols + pad), dtype=torch.int8, device=device)
-    return t[:, :cols] if pad else t
+    if not pad:
+        return torch.empty((rows, cols), dtype=torch.int8, device=device)
+    return torch.empty((rows, cols + pad), dtype=torch.int8, device=device)[:, :cols]
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
@@ -28,15 +29,9 @@ def _rows2d(t: torch.Tensor) -> torch.Tensor:
     return t if t.stride(1) == 1 or t.shape[1] <= 1 else t.contiguous()
 
 
-def _no_grad(*tensors) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _no_gradient() -> None:
+    if torch.is_grad_enabled():
         raise RuntimeError("the int8 operators have no gradient: call them under torch.no_grad()")
-
-
-def _same_device(x: torch.Tensor, **others) -> None:
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            raise ValueError(f"{name} is on {t.device}, the input on {x.device}")
 
 
 def _steps(t: torch.Tensor, amax: torch.Tensor) -> torch.Tensor:
@@ -50,35 +45,40 @@ def _ref_rows(t: torch.Tensor, norm=None):
     return _steps(t, amax), scale.squeeze(-1).float()
 
 
-def _kind(t: torch.Tensor, what: str) -> int:
-    if t.dtype == torch.bfloat16:
-        return 1
-    if t.dtype == torch.float32:
-        return 0
-    raise TypeError(f"{what} must be bf16 or fp32 on a GPU, not {t.dtype}")
+_KINDS = {torch.bfloat16: 1, torch.float32: 0}
+
+
+def _kind(dtype: torch.dtype, what: str) -> int:
+    k = _KINDS.get(dtype)
+    if k is None:
+        raise TypeError(f"{what} must be bf16 or fp32 on a GPU, not {dtype}")
+    return k
 
 
 def _launch_rows(mode: int, x: torch.Tensor, D: int, res=None, weight=None, eps: float = 0.0):
-    x2 = _rows2d(x)
-    rows, shape, dev = x2.shape[0], x.shape[:-1], x.device
-    kind = _kind(x, "x")
+    flat = x.dim() == 2
+    x2 = x if flat and x.stride(1) == 1 else _rows2d(x)
+    rows, dev, dtype = x2.shape[0], x.device, x.dtype
+    wk = kind = _kind(dtype, "x")
     q = _aligned_rows(rows, D, dev)
     scale = torch.empty(rows, dtype=torch.float32, device=dev)
-    h, rp, rs, hp, wp, wk = None, 0, 0, 0, 0, kind
+    h, rp, rs, hp, wp = None, 0, 0, 0, 0
     if weight is not None:
-        if weight.dtype != torch.float32 and weight.dtype != x.dtype:
+        if weight.dtype != torch.float32 and weight.dtype != dtype:
             weight = weight.float()
-        weight = weight.contiguous()
-        wp, wk = weight.data_ptr(), _kind(weight, "weight")
+        if not weight.is_contiguous():
+            weight = weight.contiguous()
+        wp, wk = weight.data_ptr(), _kind(weight.dtype, "weight")
     if res is not None:
-        r2 = _rows2d(res)
-        h = torch.empty((rows, D), dtype=x.dtype, device=dev)
+        r2 = res if flat and res.stride(1) == 1 else _rows2d(res)
+        h = torch.empty((rows, D), dtype=dtype, device=dev)
         rp, rs, hp = r2.data_ptr(), r2.stride(0), h.data_ptr()
     if rows:
-        N.launch("ax_int8_rows", dev, mode, kind, wk, x2.data_ptr(), x2.stride(0), rp, rs, wp, eps, hp, D, q.data_ptr(), q.stride(0),
+        N.launch("ax_int8_rows", dev.index, mode, kind, wk, x2.data_ptr(), x2.stride(0), rp, rs, wp, eps, hp, D, q.data_ptr(), q.stride(0),
                  scale.data_ptr(), rows, D)
-    if x.dim() != 2:
-        q, scale = q.unflatten(0, shape), scale.view(shape)
+    if not flat:
+        lead = x.shape[:-1]
+        q, scale = q.unflatten(0, lead), scale.view(lead)
         h = h.view(x.shape) if h is not None else None
     return q, scale, h
 
@@ -88,13 +88,14 @@ def _check_rows(x: torch.Tensor) -> None:
         raise ValueError(f"rows [..., D] with D > 0 are needed, not {tuple(x.shape)}")
     if not x.is_floating_point():
         raise TypeError(f"x must be a floating tensor, not {x.dtype}")
+    if x.requires_grad:
+        _no_gradient()
 
 
 def quantize_int8(x: torch.Tensor):
     """``x[..., K]`` to int8 rows: ``(q [..., K], scale [...])``.  For a weight ``[N, K]`` these are its
     channels.  Rows of ``q`` start on 16-byte boundaries."""
     _check_rows(x)
-    _no_grad(x)
     if not x.is_cuda:
         return _ref_rows(x.float())
     return _launch_rows(0, x, x.shape[-1])[:2]
@@ -104,14 +105,20 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
     """RMSNorm over the last dim, to int8 rows: ``(q, scale)``.  With ``residual`` the norm is of
     ``h = x + residual`` (rounded to ``x``'s type) and the result is ``(q, scale, h)``."""
     _check_rows(x)
-    _no_grad(x, weight, residual)
-    _same_device(x, weight=weight, residual=residual)
-    if weight.shape != x.shape[-1:]:
-        raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {x.shape[-1]}")
-    if residual is not None and (residual.shape != x.shape or residual.dtype != x.dtype):
-        raise ValueError("residual must have x's shape and type")
+    D, dev = x.shape[-1], x.device
+    if weight.dim() != 1 or weight.shape[0] != D:
+        raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {D}")
+    if weight.device != dev:
+        raise ValueError(f"weight is on {weight.device}, x on {dev}")
+    if weight.requires_grad:
+        _no_gradient()
+    if residual is not None:
+        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+            raise ValueError("residual must have x's shape, type and device")
+        if residual.requires_grad:
+            _no_gradient()
     if x.is_cuda:
-        q, scale, h = _launch_rows(1, x, x.shape[-1], residual, weight, eps)
+        q, scale, h = _launch_rows(1, x, D, residual, weight, eps)
     else:
         h = x if residual is None else x + residual
         hf = h.float()
@@ -122,10 +129,9 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
 def swiglu_int8(gate_up: torch.Tensor):
     """``silu(gate) * up`` of a fused ``[..., 2F]`` tensor laid out gate|up, to int8 rows ``(q, scale)``."""
     _check_rows(gate_up)
-    _no_grad(gate_up)
-    if gate_up.shape[-1] % 2:
+    F, odd = divmod(gate_up.shape[-1], 2)
+    if odd:
         raise ValueError("gate|up needs an even last dim")
-    F = gate_up.shape[-1] // 2
     if gate_up.is_cuda:
         return _launch_rows(2, gate_up, F)[:2]
     g, u = gate_up.float().split(F, dim=-1)
@@ -146,36 +152,53 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     on 16-byte boundaries are copied first; ``quantize_int8`` and the fused producers lay them out so."""
     if q.dtype != torch.int8 or weight.dtype != torch.int8:
         raise TypeError("q and weight must be int8")
+    lead = q.shape[:-1]
     if weight.dim() != 2 or q.dim() < 1 or q.shape[-1] != weight.shape[1]:
         raise ValueError(f"q {tuple(q.shape)} does not fit a weight {tuple(weight.shape)}")
     Nn, K = weight.shape
     if not 0 < K <= MAX_K:
         raise ValueError(f"K must be in 1..{MAX_K}, not {K}")
-    if scale.shape != q.shape[:-1] or weight_scale.shape != (Nn,):
+    if scale.shape != lead or weight_scale.dim() != 1 or weight_scale.shape[0] != Nn:
         raise ValueError(f"scales {tuple(scale.shape)}, {tuple(weight_scale.shape)} do not fit {tuple(q.shape)}, {tuple(weight.shape)}")
     if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
         raise TypeError("scales must be fp32")
-    if out_dtype not in (torch.bfloat16, torch.float32):
+    if out_dtype not in _KINDS:
         raise TypeError(f"out_dtype must be bf16 or fp32, not {out_dtype}")
-    if bias is not None and bias.shape != (Nn,):
-        raise ValueError(f"bias {tuple(bias.shape)} does not fit {Nn} channels")
-    _same_device(q, scale=scale, weight=weight, weight_scale=weight_scale, bias=bias)
-    _no_grad(scale, weight_scale, bias)
-    lead = q.shape[:-1]
-    q2 = q.reshape(-1, K) if q.dim() != 2 else q
+    dev = q.device
+    if bias is not None:
+        if bias.dim() != 1 or bias.shape[0] != Nn or bias.device != dev:
+            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not fit {Nn} channels on {dev}")
+        if bias.requires_grad:
+            _no_gradient()
+    if scale.device != dev or weight.device != dev or weight_scale.device != dev:
+        raise ValueError(f"q is on {dev}, its scale on {scale.device}, the weight on {weight.device}, its scale on {weight_scale.device}")
+    if scale.requires_grad or weight_scale.requires_grad:
+        _no_gradient()
+    q2 = q if q.dim() == 2 else q.reshape(-1, K)
     if not q.is_cuda:
         y = (q2.double() @ weight.double().t()).float() * scale.reshape(-1, 1) * weight_scale
         y = y if bias is None else y + bias.float()
         return y.to(out_dtype).view(*lead, Nn)
     M = q2.shape[0]
-    out = torch.empty((M, Nn), dtype=out_dtype, device=q.device)
+    out = torch.empty((M, Nn), dtype=out_dtype, device=dev)
     if M and Nn:
-        q2, w2 = _gemm_rows(q2), _gemm_rows(weight)
-        s, ws = scale.contiguous(), weight_scale.contiguous()
-        b = bias.float().contiguous() if bias is not None else None
-        N.launch("ax_int8_gemm", q.device, q2.data_ptr(), q2.stride(0), s.data_ptr(), w2.data_ptr(), w2.stride(0), ws.data_ptr(),
-                 b.data_ptr() if b is not None else 0, out.data_ptr(), Nn, int(out_dtype == torch.bfloat16), M, Nn, K,
-                 N.status_ptr(q.device))
+        qs, ws = q2.stride(0), weight.stride(0)
+        if q2.stride(1) != 1 or qs % 16 or q2.data_ptr() % 16:
+            q2 = _aligned_rows(M, K, dev).copy_(q2)
+            qs = q2.stride(0)
+        if weight.stride(1) != 1 or ws % 16 or weight.data_ptr() % 16:
+            weight = _aligned_rows(Nn, K, dev).copy_(weight)
+            ws = weight.stride(0)
+        if not scale.is_contiguous():
+            scale = scale.contiguous()
+        if not weight_scale.is_contiguous():
+            weight_scale = weight_scale.contiguous()
+        b = 0
+        if bias is not None:
+            bias = bias.float().contiguous()
+            b = bias.data_ptr()
+        N.launch("ax_int8_gemm", dev.index, q2.data_ptr(), qs, scale.data_ptr(), weight.data_ptr(), ws, weight_scale.data_ptr(), b,
+                 out.data_ptr(), Nn, _KINDS[out_dtype], M, Nn, K, N.status_ptr(dev.index))
     return out if q.dim() == 2 else out.view(*lead, Nn)
 
 

@@ -3,6 +3,7 @@ attention through a block table; the same over a cache held in int8 with one mag
 and head (``csrc/kernels/paged_int8.cu``).  CPU tensors use the same maths with torch ops."""
 from __future__ import annotations
 
+import functools
 import math
 
 import torch
@@ -80,17 +81,16 @@ def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
         raise TypeError("k_amax and v_amax must be fp32")
     if block_table.dim() != 2 or block_table.dtype != torch.int32:
         raise TypeError("block_table must be int32 [B, max_pages]")
-    for t in (k_cache, v_cache, k_amax, v_amax):
-        if not t.is_contiguous():
-            raise ValueError("the caches and their magnitudes must be contiguous")
-    for t in (v_cache, k_amax, v_amax, block_table):
-        if t.device != k_cache.device:
-            raise ValueError("the caches, their magnitudes and the block table must be on one device")
+    if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_amax.is_contiguous() and v_amax.is_contiguous()):
+        raise ValueError("the caches and their magnitudes must be contiguous")
+    dev = k_cache.device
+    if v_cache.device != dev or k_amax.device != dev or v_amax.device != dev or block_table.device != dev:
+        raise ValueError("the caches, their magnitudes and the block table must be on one device")
     return pages, Hkv, P, D
 
 
 def _int32_vector(t, n: int, name: str, device):
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device:
+    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device:
         raise ValueError(f"{name} must be int32 [{n}] on {device}")
     return t if t.is_contiguous() else t.contiguous()
 
@@ -125,12 +125,14 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
     if T == 0 or B == 0:
         return
     vec = 16 // k.element_size()
-    k, v = (t if t.stride(2) == 1 and t.stride(0) % vec == 0 and t.stride(1) % vec == 0 and t.data_ptr() % 16 == 0 else t.contiguous()
-            for t in (k, v))
+    if k.stride(2) != 1 or k.stride(0) % vec or k.stride(1) % vec or k.data_ptr() % 16:
+        k = k.clone(memory_format=torch.contiguous_format)
+    if v.stride(2) != 1 or v.stride(0) % vec or v.stride(1) % vec or v.data_ptr() % 16:
+        v = v.clone(memory_format=torch.contiguous_format)
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    N.launch("ax_kv_write_int8", k.device, int(k.dtype == torch.bfloat16), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
+    N.launch("ax_kv_write_int8", k.device.index, int(k.dtype == torch.bfloat16), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
              v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(), v_amax.data_ptr(), table.data_ptr(), starts.data_ptr(),
-             cu_seqlens.data_ptr() if cu_seqlens is not None else 0, T, B, Hkv, D, P, table.shape[1], pages, N.status_ptr(k.device))
+             cu_seqlens.data_ptr() if cu_seqlens is not None else 0, T, B, Hkv, D, P, table.shape[1], pages, N.status_ptr(k.device.index))
 
 
 def _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens) -> None:
@@ -189,15 +191,21 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
     q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
+    idx, width = q.device.index, table.shape[1]
     for b0 in range(0, B, 8192):                       # the kernel keeps a running count per sequence in shared memory
         n = min(8192, B - b0)
-        with torch.cuda.device(q.device):
-            size = N.cuda().ax_decode_int8_workspace(n, Hq, Hkv, D, table.shape[1], P)
-        ws = torch.empty(size, dtype=torch.float32, device=q.device)
-        N.launch("ax_decode_int8", q.device, q[b0:].data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(), v_amax.data_ptr(),
-                 table[b0:].data_ptr(), ctx_lens[b0:].data_ptr(), out[b0:].data_ptr(), n, Hq, Hkv, D, P, table.shape[1], pages, scale,
-                 ws.data_ptr(), N.status_ptr(q.device))
+        ws = torch.empty(_int8_workspace(idx, n, Hq, Hkv, D, width, P), dtype=torch.float32, device=q.device)
+        N.launch("ax_decode_int8", idx, q.data_ptr() + b0 * Hq * D * 2, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),
+                 v_amax.data_ptr(), table.data_ptr() + b0 * width * 4, ctx_lens.data_ptr() + b0 * 4, out.data_ptr() + b0 * Hq * D * 2, n, Hq, Hkv,
+                 D, P, width, pages, scale, ws.data_ptr(), N.status_ptr(idx))
     return out
+
+
+@functools.lru_cache(maxsize=4096)
+def _int8_workspace(index: int, *shape) -> int:
+    """Floats that the attention kernel wants beside its outputs, by shape and GPU."""
+    with torch.cuda.device(index):
+        return N.cuda().ax_decode_int8_workspace(*shape)
 
 
 def _decode_attention_int8_cpu(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale):

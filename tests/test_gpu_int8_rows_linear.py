@@ -76,7 +76,7 @@ def test_rows_do_not_write_outside_their_outputs(kernel_status):
         pad = (D + 15) // 16 * 16 + 16
         buf = torch.full((rows + 2, pad), 99, dtype=torch.int8, device="cuda")
         sc = torch.full((rows + 2,), -1.0, device="cuda")
-        N.launch("ax_int8_rows", x.device, 0, 1, 1, x.data_ptr(), D, 0, 0, 0, 0.0, 0, 0, buf[1:].data_ptr(), pad, sc[1:].data_ptr(), rows, D)
+        N.launch("ax_int8_rows", x.device.index, 0, 1, 1, x.data_ptr(), D, 0, 0, 0, 0.0, 0, 0, buf[1:].data_ptr(), pad, sc[1:].data_ptr(), rows, D)
         assert buf[0].eq(99).all() and buf[-1].eq(99).all() and buf[1:-1, D:].eq(99).all()
         assert sc[0] == -1 and sc[-1] == -1
 
