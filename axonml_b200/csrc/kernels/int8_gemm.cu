@@ -39,13 +39,17 @@ __device__ __forceinline__ void umma_s8_pair(uint32_t d, uint64_t a, uint64_t b,
       "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ uint32_t ld_cluster(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+__device__ __forceinline__ int4 ld_cluster4(uint32_t addr) {
+  int4 v;
+  asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
   return v;
 }
 __device__ __forceinline__ void store_out(float* p, float v) { *p = v; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
+__device__ __forceinline__ void store_out4(float* p, float a, float b, float c, float d) { *reinterpret_cast<float4*>(p) = make_float4(a, b, c, d); }
+__device__ __forceinline__ void store_out4(__nv_bfloat16* p, float a, float b, float c, float d) {
+  *reinterpret_cast<uint2*>(p) = make_uint2(pack_bf16x2(a, b), pack_bf16x2(c, d));
+}
 
 struct GemmArgs {
   int M, N, K;
@@ -54,7 +58,7 @@ struct GemmArgs {
   const float* bias;   // [N] or null
   void* out;           // [M, N], row stride ldo
   long ldo;
-  int tma_out;         // rows of `out` start on 16-byte boundaries: tiles leave by TMA
+  int tma_out;         // rows of `out` start on 16-byte boundaries: tiles leave by TMA, channels four at a time
   int* status;
 };
 
@@ -147,10 +151,10 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
   const int row = warp * 32 + lane, n = n0 + row;
   const uint32_t t_row = tmem + ((uint32_t)(warp * 32) << 16);
   const int cols = min(BN, p.M - m0);
-  const float sw = n < p.N ? p.sw[n] : 0.f;
-  const float bias = (p.bias != nullptr && n < p.N) ? p.bias[n] : 0.f;
-  OutT* out = (OutT*)p.out + (long)m0 * p.ldo + n;
   if (S == 1) {
+    const float sw = n < p.N ? p.sw[n] : 0.f;
+    const float bias = (p.bias != nullptr && n < p.N) ? p.bias[n] : 0.f;
+    OutT* out = (OutT*)p.out + (long)m0 * p.ldo + n;
     if (ok) {
 #pragma unroll 1
       for (int c = 0; c < cols; c += 16) {
@@ -164,8 +168,9 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
       }
     }
   } else {
-    // every block leaves its partial sums in its own shared memory, [column][row]; then block r adds
-    // the columns r, r + S, ... of all of them (integers: any order gives the same sum)
+    // every block leaves its partial sums in its own shared memory, [column][row]; then a warp of block r
+    // adds whole columns r, r + S, ... of all of them, four channels a lane (integers: any order gives the
+    // same sum)
     int* red = (int*)smem;
     if (ok) {
 #pragma unroll 1
@@ -180,16 +185,38 @@ int8_stream_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_const
     __syncwarp();
     cluster_sync_all();
     if (ok) {
+      const int n4 = n0 + 4 * lane;
       uint32_t peer[8];
 #pragma unroll
-      for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(smem_u32(red + row), s) : 0;
-#pragma unroll 4
-      for (int c = rank; c < cols; c += S) {
-        int part[8];
+      for (int s = 0; s < 8; ++s) peer[s] = s < S ? mapa_shared(smem_u32(red + 4 * lane), s) : 0;
+      float sw[4], bias[4];
 #pragma unroll
-        for (int s = 0; s < 8; ++s) part[s] = s < S ? (int)ld_cluster(peer[s] + (uint32_t)(c * kRowsA * 4)) : 0;
-        const int sum = ((part[0] + part[1]) + (part[2] + part[3])) + ((part[4] + part[5]) + (part[6] + part[7]));
-        if (n < p.N) store_out(out + (long)c * p.ldo, __int2float_rn(sum) * __ldg(p.sx + m0 + c) * sw + bias);
+      for (int j = 0; j < 4; ++j) {
+        sw[j] = n4 + j < p.N ? p.sw[n4 + j] : 0.f;
+        bias[j] = (p.bias != nullptr && n4 + j < p.N) ? p.bias[n4 + j] : 0.f;
+      }
+#pragma unroll 4
+      for (int c = rank + S * warp; c < cols; c += 4 * S) {
+        int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+          if (s < S) {
+            const int4 v = ld_cluster4(peer[s] + (uint32_t)(c * kRowsA * 4));
+            sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+          }
+        }
+        const float sx = __ldg(p.sx + m0 + c);
+        const float y0 = __int2float_rn(sum.x) * sx * sw[0] + bias[0], y1 = __int2float_rn(sum.y) * sx * sw[1] + bias[1];
+        const float y2 = __int2float_rn(sum.z) * sx * sw[2] + bias[2], y3 = __int2float_rn(sum.w) * sx * sw[3] + bias[3];
+        OutT* o = (OutT*)p.out + (long)(m0 + c) * p.ldo + n4;
+        if (p.tma_out && n4 + 3 < p.N) {      // rows on 16-byte boundaries: four channels are one store
+          store_out4(o, y0, y1, y2, y3);
+        } else {
+          if (n4 < p.N) store_out(o, y0);
+          if (n4 + 1 < p.N) store_out(o + 1, y1);
+          if (n4 + 2 < p.N) store_out(o + 2, y2);
+          if (n4 + 3 < p.N) store_out(o + 3, y3);
+        }
       }
     }
     __syncwarp();
@@ -496,26 +523,60 @@ int launch_pair(const void* q, long ldq, const void* w, long ldw, const GemmArgs
   return axh::launch_chained(kern, dim3(2 * pairs), dim3(kThreads), C::kSmem, 2, stream, mx, mw, mo, p);
 }
 
+// Which kernel, token tile and split of K: the lowest estimated time in microseconds.  The constants are fits to
+// timings of all forms at 1 to 1024 rows, 1000 to 28672 channels and K of 1024 to 14336 (a chain of
+// products, inputs larger than L2); they name what each form waits for:
+//   stream  4 to start and end; then the slowest of its k blocks in turn (0.27 each, and 4 more for every
+//           wave once there are two), shared-memory fills at 16 TB/s over all blocks, the weight at 6.3 TB/s; 0.03 a column to
+//           store, or 1 + 0.015 a column to hand over and 0.04 a column to add and store when K is split.
+//           Measured 1 x 6144 x 4096: 12.7 / 9.3 / 8.3 / 13.6 us with K split 1 / 2 / 4 / 8 ways;
+//           128 x 4096 x 4096: 14.4 / 11.7 / 9.6 us with 64 tokens and 1 / 2 / 4 ways, 15.0 as pairs.
+//   pair    0.3 a k block and wave.  512 x 28672 x 4096: 51 us as 256 x 256 tiles, 74 as 256 x 128, 90 streamed;
+//           512 x 4096 x 4096: 16.5 / 15.4 / 18.1.
+struct Choice { int bn, split; bool pair; };
+Choice choose(int M, int N, int K, int pairs) {
+  const double kb = (K + kBytesK - 1) / kBytesK, slots = 2.0 * axh::sm_count();
+  Choice best{256, 1, true};
+  double least = 1e30;
+  auto waves = [](double tiles, double room) { return (double)(long)((tiles + room - 1) / room); };
+  if (pairs > 0) {
+    const double mb = (M + 255) / 256;
+    const double t256 = 6.0 + waves(mb * ((N + 255) / 256), pairs) * (0.3 * kb + 1.6);
+    const double t128 = 5.0 + waves(mb * ((N + 127) / 128), pairs) * (0.3 * kb + 0.4);
+    least = t256 < t128 ? t256 : t128;
+    if (t128 < t256) best.bn = 128;
+  }
+  for (int bn = 16; bn <= 128; bn *= 2) {
+    if (bn > 16 && M <= bn / 2) break;
+    const double tiles = (double)((N + kRowsA - 1) / kRowsA) * ((M + bn - 1) / bn);
+    for (int S = 1; S <= 8 && S <= (int)kb; S *= 2) {
+      const double w = waves(tiles * S, slots), each = (kb + S - 1) / S;
+      const double end = S == 1 ? 0.03 * bn : 1.0 + 0.015 * bn + 0.04 * bn / S;
+      double body = w > 1 ? w * (0.3 * each + 4.0 + end) : 0.27 * each;
+      const double fill = tiles * kb * kBytesK * (kRowsA + bn) / 16.0e6, weight = (double)N * K / 6.3e6;
+      if (fill > body) body = fill;
+      if (weight > body) body = weight;
+      const double t = 4.0 + body + end;
+      if (t < least) { least = t; best = Choice{bn, S, false}; }
+    }
+  }
+  return best;
+}
+
 template <typename OutT>
 int dispatch(const void* q, long ldq, const void* w, long ldw, const GemmArgs& p, cudaStream_t stream) {
-  if (p.M <= 128) {
-    // K is split until the blocks fill the device twice over, but not below four k blocks each
-    const int tiles = (p.N + kRowsA - 1) / kRowsA, num_kb = (p.K + kBytesK - 1) / kBytesK;
-    int S = 1;
-    while (S < 8 && tiles * S * 2 <= 2 * axh::sm_count() && num_kb >= S * 2 * 4) S *= 2;
-    if (p.M <= 16) return launch_stream<16, OutT>(q, ldq, w, ldw, p, S, stream);
-    if (p.M <= 32) return launch_stream<32, OutT>(q, ldq, w, ldw, p, S, stream);
-    if (p.M <= 64) return launch_stream<64, OutT>(q, ldq, w, ldw, p, S, stream);
-    return launch_stream<128, OutT>(q, ldq, w, ldw, p, S, stream);
-  }
   const int pairs = launch_pair<256, OutT>(q, ldq, w, ldw, p, stream, true);
-  if (pairs < 1) return pairs ? pairs : -3;
-  auto waves = [&](int bn) {
-    const long tiles = (long)((p.M + 255) / 256) * ((p.N + bn - 1) / bn);
-    return (double)((tiles + pairs - 1) / pairs);
-  };
-  if (waves(256) * 1.2 <= waves(128)) return launch_pair<256, OutT>(q, ldq, w, ldw, p, stream, false);
-  return launch_pair<128, OutT>(q, ldq, w, ldw, p, stream, false);
+  const Choice c = choose(p.M, p.N, p.K, pairs);
+  if (c.pair) {
+    if (pairs < 1) return pairs ? pairs : -3;
+    return c.bn == 256 ? launch_pair<256, OutT>(q, ldq, w, ldw, p, stream, false) : launch_pair<128, OutT>(q, ldq, w, ldw, p, stream, false);
+  }
+  switch (c.bn) {
+    case 16: return launch_stream<16, OutT>(q, ldq, w, ldw, p, c.split, stream);
+    case 32: return launch_stream<32, OutT>(q, ldq, w, ldw, p, c.split, stream);
+    case 64: return launch_stream<64, OutT>(q, ldq, w, ldw, p, c.split, stream);
+    default: return launch_stream<128, OutT>(q, ldq, w, ldw, p, c.split, stream);
+  }
 }
 
 }  // namespace
