@@ -249,12 +249,19 @@ __global__ void __launch_bounds__(2 * kHalf) kv_write_int8_kernel(const WriteArg
 // batch, counted over sequences, KV heads and tokens in that order, whatever the context lengths are.
 // Its tiles arrive in a ring of stages in shared memory, K and V of a tile by one bulk copy each, several
 // tiles ahead; page numbers and magnitudes of 32 tiles are fetched by the 32 lanes at once, a batch ahead.
-// The query heads of a KV head are the rows of mma.m16n8k16 (fp16 operands, fp32 sums):
-//   S[heads x 16] = Q K^T, then O[heads x D] = alpha O + a_v / 127 (P V)
+//
+// Products (mma.m16n8k16, fp16 operands, fp32 sums), the cache on the 16-row side so that no row is idle
+// with up to eight query heads on the other:
+//   S^T[16 tokens x heads] = K Q^T,      O^T[16 dims x heads] += V^T P^T for each 16 dims
 // int8 becomes fp16 exactly (byte | 0x6400 is 1024 + byte).  Q is scaled by a power of two to lie near one,
-// where fp16 holds every bf16 significand; P in [0, 1] is rounded to fp16 (2^-11), below bf16's own rounding
-// of the result.  A worker writes a head's result itself when all its tokens were in the worker's share,
-// and otherwise a partial (O, maximum, sum) that a second kernel merges.
+// where fp16 holds every bf16 significand.  P, rounded to fp16 (2^-11, below bf16's own rounding of the
+// result), carries the page's V magnitude relative to the largest one met so far, so that O stays in the
+// accumulators; a page below 1/8 of that is summed apart and added in fp32.
+// The running maximum only moves when a score exceeds it by 2^8 (a vote of the warp finds out): weights up to 256
+// are as exact in fp16 and fp32 as weights up to one, and the usual tile needs no exchange and no rescaling.
+//
+// A worker writes a head's result itself when all its tokens were in the worker's share, and otherwise a
+// partial (O, maximum, sum) that a second kernel merges.
 constexpr int kWarps = 4;
 constexpr int kTile = 16;
 
@@ -290,10 +297,10 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
                "l"((uint64_t)src), "r"(bytes), "r"(smem_u32(bar))
                : "memory");
 }
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+               : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // Four int8 to two fp16 pairs: the byte with its sign bit flipped is value + 128; over 0x64 it is 1024 + that.
 __device__ __forceinline__ void int8x4_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
@@ -308,21 +315,30 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 v = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&v);
 }
+// Transposes an 8 x 8 matrix of 16-bit values spread over the warp (lane 4 r + c holds columns 2 c, 2 c + 1 of row r).
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
 
 template <int D>
 struct AttnCfg {
   static constexpr int kStage = 2 * kTile * D;                   // K and V of a tile
-  static constexpr int kStages = D == 64 ? 8 : (D == 128 ? 4 : 3);
+  static constexpr int kStages = D == 64 ? 6 : 3;
   static constexpr int kRing = kWarps * kStages * kStage;
-  static constexpr int kBlocks = D == 256 ? 2 : 3;               // blocks per SM that registers and shared memory allow
+  static constexpr int kBlocks = D == 256 ? 2 : 4;               // blocks per SM that registers and shared memory allow
 };
+constexpr float kSlack = 8.f;                                    // log2 of the largest weight
+constexpr float kFaint = 1.f / 8.f;
 
-template <int D, int HG>
-__global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_kernel(const AttnArgs a) {
+// NB: blocks of eight query heads.
+template <int D, int NB>
+__global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2) decode_int8_kernel(const AttnArgs a) {
   using C = AttnCfg<D>;
+  constexpr int HG = 8 * NB;
   constexpr int NJ = D / 64;                                     // 64-dim groups: a lane's 16-byte pieces of a K row
-  constexpr int NT = D / 8;                                      // 8-dim tiles of O
-  constexpr int R = HG / 8;                                      // rows of the MMA a lane owns
+  constexpr int MT = D / 16;                                     // 16-dim tiles of O^T
   extern __shared__ __align__(128) uint8_t smem[];
   uint64_t* bars = (uint64_t*)(smem + C::kRing);
   volatile int* dead = (volatile int*)(bars + kWarps * C::kStages);
@@ -368,9 +384,9 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
     }
     return lo;
   };
-  // what lane l knows about tile (batch + l): where its bytes lie, and its magnitudes
-  auto load_ids = [&](int t0, long& off, int& group) {
-    off = -1;
+  // what lane l knows about tile (t0 + l): where its bytes lie (in tiles; -1: no such page), and its magnitudes
+  auto load_ids = [&](int t0, int& at, int& group) {
+    at = -1;
     group = -1;
     if (t0 + lane < n) {
       const int f = f0 + t0 + lane, b = find_seq(f), tb = prefix[b + 1] - prefix[b], r = f - prefix[b] * VH;
@@ -380,26 +396,25 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
         set_status(a.status, kBadArgument, 1211);
       } else {
         group = page * a.Hkv + vh / a.nblk;
-        off = ((long)group * a.P + tok % a.P) * D;
+        at = group * (a.P / kTile) + (tok % a.P) / kTile;
       }
     }
   };
   auto load_amax = [&](int group, float& ka, float& va) {
-    ka = group >= 0 ? a.ka[group] : 0.f;
+    ka = group >= 0 ? a.ka[group] : -1.f;                        // negative: the tile is masked
     va = group >= 0 ? a.va[group] : 0.f;
   };
-  long off_c, off_n = -1;
-  int grp_c, grp_n = -1;
-  float ka_c, va_c, ka_n = 0.f, va_n = 0.f;
-  load_ids(0, off_c, grp_c);
-  load_amax(grp_c, ka_c, va_c);
-  auto issue = [&](int t, long off) {                            // tile t of this worker into its stage
+  int at_c, at_n = -1, grp = -1;
+  float ka_c, va_c, ka_n = -1.f, va_n = 0.f;
+  load_ids(0, at_c, grp);
+  load_amax(grp, ka_c, va_c);
+  auto issue = [&](int s, int at) {                              // a tile into stage s
     if (lane == 0) {
-      const int s = t % C::kStages;
-      if (off < 0) {
-        mbar_arrive(&full[s]);                                   // no such page: nothing is fetched, the tile is masked
+      if (at < 0) {
+        mbar_arrive(&full[s]);                                   // nothing is fetched
       } else {
         uint8_t* dst = ring + s * C::kStage;
+        const long off = (long)at * (kTile * D);
         mbar_expect_tx(&full[s], C::kStage);
         bulk_load(dst, a.kc + off, kTile * D, &full[s]);
         bulk_load(dst + kTile * D, a.vc + off, kTile * D, &full[s]);
@@ -407,166 +422,249 @@ __global__ void __launch_bounds__(kWarps * 32, AttnCfg<D>::kBlocks) decode_int8_
     }
   };
 #pragma unroll 1
-  for (int t = 0; t < C::kStages && t < n; ++t) issue(t, __shfl_sync(0xffffffffu, off_c, t));
+  for (int t = 0; t < C::kStages && t < n; ++t) issue(t, __shfl_sync(0xffffffffu, at_c, t));
 
   const int g = lane >> 2, i4 = lane & 3;
   int b = find_seq(f0), tb = prefix[b + 1] - prefix[b];
   int vh = (f0 - prefix[b] * VH) / tb, tile = f0 - prefix[b] * VH - vh * tb;
-  int ctx = 0;
-  uint32_t qa[NJ * 4][2 * R];
-  float qs[R], m[R], l[R], o[NT][2 * R];
+  int ctx = 0, s = 0;
+  uint32_t ph = 0;
+  uint32_t qb[NB][NJ * 4][2];                                    // Q^T: head g of each block, four dims a step
+  // of heads 2 i4 and 2 i4 + 1: scale, running maximum, this lane's share of the sum
+  float qs[NB][2], m[NB][2], l[NB][2], o[NB][MT][4];
+  float vref = 0.f, vinv = 1.f;                                  // V magnitude (/ 127) that O is counted in, and 1 / it
   bool fresh = true;
 
 #pragma unroll 1
   for (int t = 0; t < n; ++t) {
     const int bi = t & 31;
     if (bi == 0) {
-      if (t > 0) { off_c = off_n; grp_c = grp_n; ka_c = ka_n; va_c = va_n; }
-      if (t + 32 < n) load_ids(t + 32, off_n, grp_n);
+      if (t > 0) { at_c = at_n; ka_c = ka_n; va_c = va_n; }
+      if (t + 32 < n) load_ids(t + 32, at_n, grp);
     }
-    if (bi == 8 && t - 8 + 32 < n) load_amax(grp_n, ka_n, va_n);
+    if (bi == 8 && t - 8 + 32 < n) load_amax(grp, ka_n, va_n);
     if (fresh) {
       fresh = false;
       ctx = min(a.ctx[b], a.max_pages * a.P);
       const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        const bool live = first + g + 8 * r < a.G;
-        const __nv_bfloat16* qp = a.q + ((long)b * a.Hq + h0 + first + g + 8 * r) * D;
-        float v[NJ][16];
+      for (int nb = 0; nb < NB; ++nb) {
+        const int head = first + 8 * nb + g;
+        const bool live = head < a.G;
+        const __nv_bfloat16* qp = a.q + ((long)b * a.Hq + h0 + head) * D;
+        Raw8<__nv_bfloat16> raw[NJ][2];
         float top = 0.f;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          float x0[8], x1[8];
-          if (live) {
-            Raw8<__nv_bfloat16> q0, q1;
-            q0.load(qp + (i4 + 4 * j) * 16);
-            q1.load(qp + (i4 + 4 * j) * 16 + 8);
-            q0.get(x0);
-            q1.get(x1);
-          }
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            v[j][e] = live ? x0[e] : 0.f;
-            v[j][8 + e] = live ? x1[e] : 0.f;
-            top = fmaxf(top, fmaxf(fabsf(v[j][e]), fabsf(v[j][8 + e])));
-          }
-        }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two at or below the row's largest value (clamped: its inverse is a normal number too)
-        const uint32_t e = min(max(__float_as_uint(top) >> 23, 2u), 252u);
-        qs[r] = __uint_as_float(e << 23) * a.scale_log2;
-        const float down = __uint_as_float((254u - e) << 23);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            qa[j * 4 + k][r] = pack_half2(v[j][4 * k] * down, v[j][4 * k + 1] * down);
-            qa[j * 4 + k][R + r] = pack_half2(v[j][4 * k + 2] * down, v[j][4 * k + 3] * down);
+          for (int e = 0; e < 2; ++e) {
+            raw[j][e].u = make_uint4(0u, 0u, 0u, 0u);
+            if (live) raw[j][e].load(qp + (i4 + 4 * j) * 16 + 8 * e);
           }
-        m[r] = -INFINITY;
-        l[r] = 0.f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v[8];
+            raw[j][e].get(v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+          }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        // the power of two at or below the head's largest value (clamped: its inverse is a normal number too);
+        // a negative scale goes into Q, so that the factor of the scores is never negative
+        const uint32_t e2 = min(max(__float_as_uint(top) >> 23, 2u), 252u);
+        const float scale = __uint_as_float(e2 << 23) * fabsf(a.scale_log2);
+        const float down = copysignf(__uint_as_float((254u - e2) << 23), a.scale_log2);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float v[8];
+            raw[j][e].get(v);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              qb[nb][j * 4 + 2 * e + k][0] = pack_half2(v[4 * k] * down, v[4 * k + 1] * down);
+              qb[nb][j * 4 + 2 * e + k][1] = pack_half2(v[4 * k + 2] * down, v[4 * k + 3] * down);
+            }
+          }
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          qs[nb][c] = __shfl_sync(0xffffffffu, scale, (2 * i4 + c) * 4);
+          m[nb][c] = -INFINITY;
+          l[nb][c] = 0.f;
+        }
+#pragma unroll
+        for (int x = 0; x < MT; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.f;
       }
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int y = 0; y < 2 * R; ++y) o[x][y] = 0.f;
+      vref = 0.f;
+      vinv = 1.f;
     }
-    const int s = t % C::kStages;
-    bool ok = mbar_wait(&full[s], (uint32_t)((t / C::kStages) & 1), dead, a.status, 1212);
+    bool ok = mbar_wait(&full[s], ph, dead, a.status, 1212);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok) break;
     const uint8_t* kt = ring + s * C::kStage;
     const uint8_t* vt = kt + kTile * D;
     const float ka = __shfl_sync(0xffffffffu, ka_c, bi), va = __shfl_sync(0xffffffffu, va_c, bi) * (1.f / 127.f);
-    const bool have = __shfl_sync(0xffffffffu, grp_c, bi) >= 0;
-    const int left = have ? ctx - tile * kTile : 0;              // tokens of the tile that count
+    const int left = ka < 0.f ? 0 : ctx - tile * kTile;          // tokens of the tile that count (a NaN magnitude counts)
 
-    // ---- S: column c of 8-token tile nt is token 4 (c / 2) + c % 2 + 2 nt, so that the lane's four scores are tokens 4 i4 ..
-    float sc[2][4];
+    // ---- S^T: row r of the MMA is token 4 (r / 2 % 4) + r % 2 + 2 (r / 8), so that after the transposition below a lane
+    // has the weights of tokens 4 i4 .. 4 i4 + 3, whose V bytes are one word
+    float sc[NB][4];
 #pragma unroll
-    for (int nt = 0; nt < 2; ++nt) {
-      sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-      const uint8_t* row = kt + (4 * (g >> 1) + (g & 1) + 2 * nt) * D;
+    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+    const int tok = 4 * (g >> 1) + (g & 1);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const uint4 kk = *reinterpret_cast<const uint4*>(row + (i4 + 4 * j) * 16);
-        const uint32_t kw[4] = {kk.x, kk.y, kk.z, kk.w};
+    for (int j = 0; j < NJ; ++j) {
+      const uint4 k0 = *reinterpret_cast<const uint4*>(kt + tok * D + (i4 + 4 * j) * 16);
+      const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (tok + 2) * D + (i4 + 4 * j) * 16);
+      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t b0, b1;
-          int8x4_to_half(kw[k], b0, b1);
-          const int x = j * 4 + k;
-          if (R == 1) mma_f16(sc[nt], qa[x][0], 0u, qa[x][1], 0u, b0, b1);
-          else mma_f16(sc[nt], qa[x][0], qa[x][1], qa[x][R], qa[x][R + (R - 1)], b0, b1);
+      for (int k = 0; k < 4; ++k) {
+        uint32_t f[4];
+        int8x4_to_half(w0[k], f[0], f[2]);
+        int8x4_to_half(w1[k], f[1], f[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_f16(sc[nb], f, qb[nb][j * 4 + k][0], qb[nb][j * 4 + k][1]);
+      }
+    }
+    if (left < kTile) {                                          // (uniform) tokens behind the context
+      const float lo = tok < left ? 0.f : -INFINITY, hi = tok + 2 < left ? 0.f : -INFINITY;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        sc[nb][0] = lo == 0.f ? sc[nb][0] : lo; sc[nb][1] = lo == 0.f ? sc[nb][1] : lo;
+        sc[nb][2] = hi == 0.f ? sc[nb][2] : hi; sc[nb][3] = hi == 0.f ? sc[nb][3] : hi;
+      }
+    }
+    // ---- weights.  Column c of sc is head 2 i4 + c % 2.
+    bool move = va > vref;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float f = ka * qs[nb][c];
+        // masked scores stay -inf whatever the factor (0 x inf would be a NaN)
+        sc[nb][c] = sc[nb][c] == -INFINITY ? -INFINITY : sc[nb][c] * f;
+        sc[nb][2 + c] = sc[nb][2 + c] == -INFINITY ? -INFINITY : sc[nb][2 + c] * f;
+        move |= fmaxf(sc[nb][c], sc[nb][2 + c]) > m[nb][c] + kSlack;
+      }
+    if (__any_sync(0xffffffffu, move)) {
+      const float vnew = fmaxf(vref, va), down = vnew > 0.f ? __fdiv_rn(vref, vnew) : 1.f;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float mx = fmaxf(sc[nb][c], sc[nb][2 + c]);
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+          const float mn = mx > m[nb][c] + kSlack ? mx : m[nb][c];
+          const float alpha = m[nb][c] == -INFINITY ? 0.f : exp2f(m[nb][c] - mn);
+          m[nb][c] = mn;
+          l[nb][c] *= alpha;
+          const float all = alpha * down;
+#pragma unroll
+          for (int x = 0; x < MT; ++x) {
+            o[nb][x][c] *= all;
+            o[nb][x][2 + c] *= all;
+          }
+        }
+      vref = vnew;
+      vinv = vnew > 0.f ? __fdiv_rn(1.f, vnew) : 1.f;
+    }
+    const float ratio = va * vinv;
+    const bool faint = ratio < kFaint;                           // (uniform; a NaN magnitude is not)
+    const float pr = faint ? 1.f : ratio;
+    uint32_t pb[NB][2];
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      float pv[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float base = m[nb][c & 1] == -INFINITY ? 0.f : m[nb][c & 1];     // nothing seen yet: all weights are 0
+        pv[c] = exp2f(sc[nb][c] - base);
+      }
+      l[nb][0] += pv[0] + pv[2];
+      l[nb][1] += pv[1] + pv[3];
+      pb[nb][0] = transpose8x8(pack_half2(pv[0] * pr, pv[1] * pr));
+      pb[nb][1] = transpose8x8(pack_half2(pv[2] * pr, pv[3] * pr));
+    }
+    // ---- O^T: dims g and g + 8 of each tile, tokens 4 i4 .. 4 i4 + 3
+    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vt) + g * 4 + i4;
+    if (!faint) {
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+        uint32_t f[4];
+        int8x4_to_half(vw[x * 64], f[0], f[2]);
+        int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][x], f, pb[nb][0], pb[nb][1]);
+      }
+    } else {
+#pragma unroll
+      for (int x = 0; x < MT; ++x) {
+        uint32_t f[4];
+        int8x4_to_half(vw[x * 64], f[0], f[2]);
+        int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+          float c[4] = {0.f, 0.f, 0.f, 0.f};
+          mma_f16(c, f, pb[nb][0], pb[nb][1]);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) o[nb][x][k] += c[k] * ratio;
         }
       }
     }
-    // ---- running maximum and sum
-    uint32_t pa[2][2];                                           // [row][tokens 4 i4, +1 | +2, +3]
-    float alpha[R];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const float f = ka * qs[r];
-      float sv[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) sv[j] = 4 * i4 + j < left ? sc[j >> 1][2 * r + (j & 1)] * f : -INFINITY;
-      float mx = fmaxf(fmaxf(sv[0], sv[1]), fmaxf(sv[2], sv[3]));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-      mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-      const float mn = fmaxf(m[r], mx);
-      const float base = mn == -INFINITY ? 0.f : mn;             // nothing seen yet: all weights are exp2(-inf) = 0
-      alpha[r] = exp2f(m[r] - base);
-      float pv[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) pv[j] = exp2f(sv[j] - base);
-      l[r] = l[r] * alpha[r] + (pv[0] + pv[1]) + (pv[2] + pv[3]);
-      m[r] = mn;
-      pa[r][0] = pack_half2(pv[0], pv[1]);
-      pa[r][1] = pack_half2(pv[2], pv[3]);
-    }
-    // ---- O
-#pragma unroll
-    for (int x = 0; x < NT; ++x) {
-      uint32_t b0, b1;
-      int8x4_to_half(*reinterpret_cast<const uint32_t*>(vt + (x * 8 + g) * 16 + i4 * 4), b0, b1);
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
-      mma_f16(c, pa[0][0], R == 2 ? pa[R - 1][0] : 0u, pa[0][1], R == 2 ? pa[R - 1][1] : 0u, b0, b1);
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        o[x][2 * r] = o[x][2 * r] * alpha[r] + c[2 * r] * va;
-        o[x][2 * r + 1] = o[x][2 * r + 1] * alpha[r] + c[2 * r + 1] * va;
-      }
-    }
     __syncwarp();                                                // the stage has been read by all lanes
-    if (t + C::kStages < n) {
+    {
       const int ahead = bi + C::kStages;
-      const long oc = __shfl_sync(0xffffffffu, off_c, ahead & 31), on = __shfl_sync(0xffffffffu, off_n, ahead & 31);
-      issue(t + C::kStages, ahead < 32 ? oc : on);
+      const int at = __shfl_sync(0xffffffffu, ahead < 32 ? at_c : at_n, ahead & 31);
+      if (t + C::kStages < n) issue(s, at);
     }
+    if (++s == C::kStages) { s = 0; ph ^= 1; }
     // ---- end of this head's tokens, or of this worker's share
     if (tile + 1 == tb || t + 1 == n) {
       const int seg = prefix[b] * VH + vh * tb;                  // flat tile the head begins with
       const bool whole = seg >= f0 && seg + tb <= f1;
       const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
 #pragma unroll
-      for (int r = 0; r < R; ++r) {
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-        l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-        const int head = first + g + 8 * r;
-        if (head < a.G) {
-          if (whole) {
-            const float inv = l[r] != 0.f ? __fdividef(1.f, l[r]) : 0.f;
-            __nv_bfloat16* op = a.out + ((long)b * a.Hq + h0 + head) * D + 2 * i4;
+      for (int nb = 0; nb < NB; ++nb) {
+        float up[2];
 #pragma unroll
-            for (int x = 0; x < NT; ++x) *reinterpret_cast<uint32_t*>(op + x * 8) = pack_bf16x2(o[x][2 * r] * inv, o[x][2 * r + 1] * inv);
-          } else {
-            const long slot = ((long)w * 2 + (seg < f0 ? 0 : 1)) * HG + g + 8 * r;
-            float* pp = a.part + slot * D + 2 * i4;
+        for (int c = 0; c < 2; ++c) {
+          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 4);
+          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 8);
+          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 16);
+          up[c] = whole ? (l[nb][c] != 0.f ? __fdividef(vref, l[nb][c]) : 0.f) : vref;
+        }
+        if (whole) {
+          // pairs of heads of a dim -> pairs of dims of a head
+          const int head = first + 8 * nb + g;
+          __nv_bfloat16* op = a.out + ((long)b * a.Hq + h0 + head) * D + 2 * i4;
 #pragma unroll
-            for (int x = 0; x < NT; ++x) *reinterpret_cast<float2*>(pp + x * 8) = make_float2(o[x][2 * r], o[x][2 * r + 1]);
-            if (i4 == 0) { a.ml[slot * 2] = m[r]; a.ml[slot * 2 + 1] = l[r]; }
+          for (int x = 0; x < MT; ++x) {
+            const uint32_t lo = transpose8x8(pack_bf16x2(o[nb][x][0] * up[0], o[nb][x][1] * up[1]));
+            const uint32_t hi = transpose8x8(pack_bf16x2(o[nb][x][2] * up[0], o[nb][x][3] * up[1]));
+            if (head < a.G) {
+              *reinterpret_cast<uint32_t*>(op + x * 16) = lo;
+              *reinterpret_cast<uint32_t*>(op + x * 16 + 8) = hi;
+            }
+          }
+        } else {
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            const int row = 8 * nb + 2 * i4 + c;
+            if (first + row < a.G) {
+              const long slot = ((long)w * 2 + (seg < f0 ? 0 : 1)) * HG + row;
+              float* pp = a.part + slot * D + g;
+#pragma unroll
+              for (int x = 0; x < MT; ++x) {
+                pp[x * 16] = o[nb][x][c] * up[c];
+                pp[x * 16 + 8] = o[nb][x][2 + c] * up[c];
+              }
+              if (g == 0) { a.ml[slot * 2] = m[nb][c]; a.ml[slot * 2 + 1] = l[nb][c]; }
+            }
           }
         }
       }
@@ -668,7 +766,7 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
 template <int D, int HG>
 int launch_attn(AttnArgs& a, int blocks, int merge_warps, cudaStream_t stream) {
   using C = AttnCfg<D>;
-  auto kern = decode_int8_kernel<D, HG>;
+  auto kern = decode_int8_kernel<D, HG / 8>;
   const int smem = C::kRing + kWarps * C::kStages * 8 + 8 + (a.B + 1) * 4;
   static int configured[64] = {0};
   int dev = 0;
@@ -706,10 +804,10 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
 }
 
 // Workers (warps) the attention kernel runs with: what fills the device, fewer for a small cache.
-static int attn_blocks(int B, int VH, int D, int max_pages, int P, int min_chunk) {
+static int attn_blocks(int B, int VH, int D, int HG, int max_pages, int P, int min_chunk) {
   const long tiles = (long)B * VH * ((long)max_pages * P / kTile);
   const long want = (tiles + (long)min_chunk * kWarps - 1) / ((long)min_chunk * kWarps);
-  const long most = (long)axh::sm_count() * (D == 256 ? 2 : 3);
+  const long most = (long)axh::sm_count() * (HG == 16 || D == 256 ? 2 : 4);
   const long few = (tiles + min_chunk - 1) / min_chunk;           // one worker a block while that spreads them further
   const long n = want < axh::sm_count() ? (few < axh::sm_count() ? few : axh::sm_count()) : want;
   return (int)(n < most ? (n > 0 ? n : 1) : most);
@@ -721,7 +819,7 @@ constexpr int kMinChunk = 4;
 AX_API long ax_decode_int8_workspace(int B, int Hq, int Hkv, int D, int max_pages, int P) {
   if (Hkv <= 0 || Hq % Hkv || P <= 0) return 0;
   const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
-  const long workers = (long)attn_blocks(B, Hkv * nblk, D, max_pages, P, kMinChunk) * kWarps;
+  const long workers = (long)attn_blocks(B, Hkv * nblk, D, HG, max_pages, P, kMinChunk) * kWarps;
   return workers * 2 * HG * (D + 2);
 }
 
@@ -735,8 +833,8 @@ AX_API int ax_decode_int8(const void* q, const int8_t* kc, const int8_t* vc, con
   if (Hkv <= 0 || Hq % Hkv || P <= 0 || P % 16 || B > 8192 || (long)B * Hq > 0x7fffffffL) return -1;
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)workspace) & 15) return -2;
   const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
-  if ((long)B * Hkv * nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv > 0x7fffffffL) return -3;
-  const int blocks = attn_blocks(B, Hkv * nblk, D, max_pages, P, kMinChunk);
+  if ((long)B * Hkv * nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv * (P / kTile) > 0x7fffffffL) return -3;
+  const int blocks = attn_blocks(B, Hkv * nblk, D, HG, max_pages, P, kMinChunk);
   const int workers = blocks * kWarps;
   AttnArgs a{(const __nv_bfloat16*)q, kc, vc, ka, va, table, ctx, (__nv_bfloat16*)out, workspace, workspace + (long)workers * 2 * HG * D,
              B, Hq, Hkv, G, nblk, P, max_pages, num_pages, kMinChunk, workers, scale * 1.4426950408889634f / 127.f, status};

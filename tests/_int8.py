@@ -73,11 +73,12 @@ def attention(q, k_rows, v_rows_, ka, va, table, ctx, scale):
         mag = torch.einsum("hgd,hnd->hgn", qq.abs(), k.abs()).amax(-1)
         tiny = qq.abs().amax(-1) * k.abs().sum(-1).amax(-1, keepdim=True)
         ds = 2 * scale * ((16 + D / 16) * 2.0 ** -22 * mag + 4 * 2.0 ** -24 * mag + 2.0 ** -24 * tiny)
-        # a weight: fp16's half step 2^-11, exp2's 2^-21, fp32 sums of them; below 2^-14 of the largest weight 2^-25 of that
+        # a weight: fp16's half step 2^-11, exp2's 2^-21, fp32 sums of them.  Below 2^-14 fp16 keeps 2^-25; the weight is stored times
+        # its page's V magnitude over the largest page's, at least 1/8, and the largest weight is at least one: 8 * 2^-25 of that
         ew = 2 * ds + 2.0 ** -11 + 2.0 ** -20
         av = torch.einsum("hgn,hnd->hgd", w, v.abs())
         top = torch.exp(s.amax(-1) - torch.logsumexp(s, -1))
-        off[b] = (ew[..., None] * av + (2.0 ** -25 * top)[..., None] * v.abs().sum(1)[:, None, :] + 2.0 ** -20 * av).reshape(Hq, D)
+        off[b] = (ew[..., None] * av + (8 * 2.0 ** -25 * top)[..., None] * v.abs().sum(1)[:, None, :] + 2.0 ** -20 * av).reshape(Hq, D)
     return out, off
 
 
