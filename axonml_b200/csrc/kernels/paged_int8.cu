@@ -330,6 +330,7 @@ struct AttnCfg {
   static constexpr int kBlocks = D == 256 ? 2 : 4;               // blocks per SM that registers and shared memory allow
 };
 constexpr float kSlack = 8.f;                                    // log2 of the largest weight
+constexpr float kNone = -1e30f;                                  // running maximum before the first score
 constexpr float kFaint = 1.f / 8.f;
 
 // NB: blocks of eight query heads.
@@ -433,261 +434,257 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
   // of heads 2 i4 and 2 i4 + 1: scale, running maximum, this lane's share of the sum
   float qs[NB][2], m[NB][2], l[NB][2], o[NB][MT][4];
   float vref = 0.f, vinv = 1.f;                                  // V magnitude (/ 127) that O is counted in, and 1 / it
-  bool fresh = true;
-
 #pragma unroll 1
-  for (int t = 0; t < n; ++t) {
-    const int bi = t & 31;
-    if (bi == 0) {
-      if (t > 0) { at_c = at_n; ka_c = ka_n; va_c = va_n; }
-      if (t + 32 < n) load_ids(t + 32, at_n, grp);
-    }
-    if (bi == 8 && t - 8 + 32 < n) load_amax(grp, ka_n, va_n);
-    if (fresh) {
-      fresh = false;
-      ctx = min(a.ctx[b], a.max_pages * a.P);
-      const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
+  for (int t = 0; t < n;) {
+    // ---- a head: all or part of its tokens
+    ctx = min(a.ctx[b], a.max_pages * a.P);
+    const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        const int head = first + 8 * nb + g;
-        const bool live = head < a.G;
-        const __nv_bfloat16* qp = a.q + ((long)b * a.Hq + h0 + head) * D;
-        Raw8<__nv_bfloat16> raw[NJ][2];
-        float top = 0.f;
+    for (int nb = 0; nb < NB; ++nb) {
+      const int head = first + 8 * nb + g;
+      const bool live = head < a.G;
+      const __nv_bfloat16* qp = a.q + ((long)b * a.Hq + h0 + head) * D;
+      Raw8<__nv_bfloat16> raw[NJ][2];
+      float top = 0.f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            raw[j][e].u = make_uint4(0u, 0u, 0u, 0u);
-            if (live) raw[j][e].load(qp + (i4 + 4 * j) * 16 + 8 * e);
-          }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v[8];
-            raw[j][e].get(v);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
-          }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        // the power of two at or below the head's largest value (clamped: its inverse is a normal number too);
-        // a negative scale goes into Q, so that the factor of the scores is never negative
-        const uint32_t e2 = min(max(__float_as_uint(top) >> 23, 2u), 252u);
-        const float scale = __uint_as_float(e2 << 23) * fabsf(a.scale_log2);
-        const float down = copysignf(__uint_as_float((254u - e2) << 23), a.scale_log2);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float v[8];
-            raw[j][e].get(v);
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              qb[nb][j * 4 + 2 * e + k][0] = pack_half2(v[4 * k] * down, v[4 * k + 1] * down);
-              qb[nb][j * 4 + 2 * e + k][1] = pack_half2(v[4 * k + 2] * down, v[4 * k + 3] * down);
-            }
-          }
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          qs[nb][c] = __shfl_sync(0xffffffffu, scale, (2 * i4 + c) * 4);
-          m[nb][c] = -INFINITY;
-          l[nb][c] = 0.f;
+        for (int e = 0; e < 2; ++e) {
+          raw[j][e].u = make_uint4(0u, 0u, 0u, 0u);
+          if (live) raw[j][e].load(qp + (i4 + 4 * j) * 16 + 8 * e);
         }
 #pragma unroll
-        for (int x = 0; x < MT; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.f;
-      }
-      vref = 0.f;
-      vinv = 1.f;
-    }
-    bool ok = mbar_wait(&full[s], ph, dead, a.status, 1212);
-    ok = __all_sync(0xffffffffu, ok);
-    if (!ok) break;
-    const uint8_t* kt = ring + s * C::kStage;
-    const uint8_t* vt = kt + kTile * D;
-    const float ka = __shfl_sync(0xffffffffu, ka_c, bi), va = __shfl_sync(0xffffffffu, va_c, bi) * (1.f / 127.f);
-    const int left = ka < 0.f ? 0 : ctx - tile * kTile;          // tokens of the tile that count (a NaN magnitude counts)
-
-    // ---- S^T: row r of the MMA is token 4 (r / 2 % 4) + r % 2 + 2 (r / 8), so that after the transposition below a lane
-    // has the weights of tokens 4 i4 .. 4 i4 + 3, whose V bytes are one word
-    float sc[NB][4];
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
-    const int tok = 4 * (g >> 1) + (g & 1);
+        for (int e = 0; e < 2; ++e) {
+          float v[8];
+          raw[j][e].get(v);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      const uint4 k0 = *reinterpret_cast<const uint4*>(kt + tok * D + (i4 + 4 * j) * 16);
-      const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (tok + 2) * D + (i4 + 4 * j) * 16);
-      const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+          for (int k = 0; k < 8; ++k) top = fmaxf(top, fabsf(v[k]));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // the power of two at or below the head's largest value (clamped: its inverse is a normal number too);
+      // a negative scale goes into Q, so that the factor of the scores is never negative
+      const uint32_t e2 = min(max(__float_as_uint(top) >> 23, 2u), 252u);
+      const float scale = __uint_as_float(e2 << 23) * fabsf(a.scale_log2);
+      const float down = copysignf(__uint_as_float((254u - e2) << 23), a.scale_log2);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        uint32_t f[4];
-        int8x4_to_half(w0[k], f[0], f[2]);
-        int8x4_to_half(w1[k], f[1], f[3]);
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma_f16(sc[nb], f, qb[nb][j * 4 + k][0], qb[nb][j * 4 + k][1]);
-      }
-    }
-    if (left < kTile) {                                          // (uniform) tokens behind the context
-      const float lo = tok < left ? 0.f : -INFINITY, hi = tok + 2 < left ? 0.f : -INFINITY;
+        for (int e = 0; e < 2; ++e) {
+          float v[8];
+          raw[j][e].get(v);
 #pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        sc[nb][0] = lo == 0.f ? sc[nb][0] : lo; sc[nb][1] = lo == 0.f ? sc[nb][1] : lo;
-        sc[nb][2] = hi == 0.f ? sc[nb][2] : hi; sc[nb][3] = hi == 0.f ? sc[nb][3] : hi;
-      }
-    }
-    // ---- weights.  Column c of sc is head 2 i4 + c % 2.
-    bool move = va > vref;
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
+          for (int k = 0; k < 2; ++k) {
+            qb[nb][j * 4 + 2 * e + k][0] = pack_half2(v[4 * k] * down, v[4 * k + 1] * down);
+            qb[nb][j * 4 + 2 * e + k][1] = pack_half2(v[4 * k + 2] * down, v[4 * k + 3] * down);
+          }
+        }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const float f = ka * qs[nb][c];
-        // masked scores stay -inf whatever the factor (0 x inf would be a NaN)
-        sc[nb][c] = sc[nb][c] == -INFINITY ? -INFINITY : sc[nb][c] * f;
-        sc[nb][2 + c] = sc[nb][2 + c] == -INFINITY ? -INFINITY : sc[nb][2 + c] * f;
-        move |= fmaxf(sc[nb][c], sc[nb][2 + c]) > m[nb][c] + kSlack;
+        qs[nb][c] = __shfl_sync(0xffffffffu, scale, (2 * i4 + c) * 4);
+        m[nb][c] = kNone;
+        l[nb][c] = 0.f;
       }
-    if (__any_sync(0xffffffffu, move)) {
-      const float vnew = fmaxf(vref, va), down = vnew > 0.f ? __fdiv_rn(vref, vnew) : 1.f;
+#pragma unroll
+      for (int x = 0; x < MT; ++x) o[nb][x][0] = o[nb][x][1] = o[nb][x][2] = o[nb][x][3] = 0.f;
+    }
+    vref = 0.f;
+    vinv = 1.f;
+    const int run = min(tb - tile, n - t);
+#pragma unroll 1
+    for (int e = 0; e < run; ++e, ++t) {
+      const int bi = t & 31;
+      if (bi == 0) {
+        if (t > 0) { at_c = at_n; ka_c = ka_n; va_c = va_n; }
+        if (t + 32 < n) load_ids(t + 32, at_n, grp);
+      }
+      if (bi == 8 && t - 8 + 32 < n) load_amax(grp, ka_n, va_n);
+      bool ok = mbar_wait(&full[s], ph, dead, a.status, 1212);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) return;
+      const uint8_t* kt = ring + s * C::kStage;
+      const uint8_t* vt = kt + kTile * D;
+      const float ka = __shfl_sync(0xffffffffu, ka_c, bi), va = __shfl_sync(0xffffffffu, va_c, bi) * (1.f / 127.f);
+      const int left = ka < 0.f ? 0 : ctx - (tile + e) * kTile;          // tokens of the tile that count (a NaN magnitude counts)
+
+      // ---- S^T: row r of the MMA is token 4 (r / 2 % 4) + r % 2 + 2 (r / 8), so that after the transposition below a lane
+      // has the weights of tokens 4 i4 .. 4 i4 + 3, whose V bytes are one word
+      float sc[NB][4];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+      const int tok = 4 * (g >> 1) + (g & 1);
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const uint4 k0 = *reinterpret_cast<const uint4*>(kt + tok * D + (i4 + 4 * j) * 16);
+        const uint4 k1 = *reinterpret_cast<const uint4*>(kt + (tok + 2) * D + (i4 + 4 * j) * 16);
+        const uint32_t w0[4] = {k0.x, k0.y, k0.z, k0.w}, w1[4] = {k1.x, k1.y, k1.z, k1.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t f[4];
+          int8x4_to_half(w0[k], f[0], f[2]);
+          int8x4_to_half(w1[k], f[1], f[3]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_f16(sc[nb], f, qb[nb][j * 4 + k][0], qb[nb][j * 4 + k][1]);
+        }
+      }
+      // ---- weights.  Column c of sc is head 2 i4 + c % 2.
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          float mx = fmaxf(sc[nb][c], sc[nb][2 + c]);
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
-          mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-          const float mn = mx > m[nb][c] + kSlack ? mx : m[nb][c];
-          const float alpha = m[nb][c] == -INFINITY ? 0.f : exp2f(m[nb][c] - mn);
-          m[nb][c] = mn;
-          l[nb][c] *= alpha;
-          const float all = alpha * down;
+        for (int c = 0; c < 4; ++c) sc[nb][c] *= ka * qs[nb][c & 1];
+      if (left < kTile) {                                        // (uniform) tokens behind the context
 #pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            o[nb][x][c] *= all;
-            o[nb][x][2 + c] *= all;
-          }
-        }
-      vref = vnew;
-      vinv = vnew > 0.f ? __fdiv_rn(1.f, vnew) : 1.f;
-    }
-    const float ratio = va * vinv;
-    const bool faint = ratio < kFaint;                           // (uniform; a NaN magnitude is not)
-    const float pr = faint ? 1.f : ratio;
-    uint32_t pb[NB][2];
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) {
-      float pv[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const float base = m[nb][c & 1] == -INFINITY ? 0.f : m[nb][c & 1];     // nothing seen yet: all weights are 0
-        pv[c] = exp2f(sc[nb][c] - base);
+          for (int c = 0; c < 4; ++c)
+            if (tok + (c & 2) >= left) sc[nb][c] = -INFINITY;
       }
-      l[nb][0] += pv[0] + pv[2];
-      l[nb][1] += pv[1] + pv[3];
-      pb[nb][0] = transpose8x8(pack_half2(pv[0] * pr, pv[1] * pr));
-      pb[nb][1] = transpose8x8(pack_half2(pv[2] * pr, pv[3] * pr));
-    }
-    // ---- O^T: dims g and g + 8 of each tile, tokens 4 i4 .. 4 i4 + 3
-    const uint32_t* vw = reinterpret_cast<const uint32_t*>(vt) + g * 4 + i4;
-    if (!faint) {
+      bool move = va > vref;
 #pragma unroll
-      for (int x = 0; x < MT; ++x) {
-        uint32_t f[4];
-        int8x4_to_half(vw[x * 64], f[0], f[2]);
-        int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
+      for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][x], f, pb[nb][0], pb[nb][1]);
-      }
-    } else {
+        for (int c = 0; c < 2; ++c) move |= fmaxf(sc[nb][c], sc[nb][2 + c]) > m[nb][c] + kSlack;
+      if (__any_sync(0xffffffffu, move)) {
+        const float vnew = fmaxf(vref, va), down = vnew > 0.f ? __fdiv_rn(vref, vnew) : 1.f;
 #pragma unroll
-      for (int x = 0; x < MT; ++x) {
-        uint32_t f[4];
-        int8x4_to_half(vw[x * 64], f[0], f[2]);
-        int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          float c[4] = {0.f, 0.f, 0.f, 0.f};
-          mma_f16(c, f, pb[nb][0], pb[nb][1]);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) o[nb][x][k] += c[k] * ratio;
-        }
-      }
-    }
-    __syncwarp();                                                // the stage has been read by all lanes
-    {
-      const int ahead = bi + C::kStages;
-      const int at = __shfl_sync(0xffffffffu, ahead < 32 ? at_c : at_n, ahead & 31);
-      if (t + C::kStages < n) issue(s, at);
-    }
-    if (++s == C::kStages) { s = 0; ph ^= 1; }
-    // ---- end of this head's tokens, or of this worker's share
-    if (tile + 1 == tb || t + 1 == n) {
-      const int seg = prefix[b] * VH + vh * tb;                  // flat tile the head begins with
-      const bool whole = seg >= f0 && seg + tb <= f1;
-      const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
-#pragma unroll
-      for (int nb = 0; nb < NB; ++nb) {
-        float up[2];
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 4);
-          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 8);
-          l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 16);
-          up[c] = whole ? (l[nb][c] != 0.f ? __fdividef(vref, l[nb][c]) : 0.f) : vref;
-        }
-        if (whole) {
-          // pairs of heads of a dim -> pairs of dims of a head
-          const int head = first + 8 * nb + g;
-          __nv_bfloat16* op = a.out + ((long)b * a.Hq + h0 + head) * D + 2 * i4;
-#pragma unroll
-          for (int x = 0; x < MT; ++x) {
-            const uint32_t lo = transpose8x8(pack_bf16x2(o[nb][x][0] * up[0], o[nb][x][1] * up[1]));
-            const uint32_t hi = transpose8x8(pack_bf16x2(o[nb][x][2] * up[0], o[nb][x][3] * up[1]));
-            if (head < a.G) {
-              *reinterpret_cast<uint32_t*>(op + x * 16) = lo;
-              *reinterpret_cast<uint32_t*>(op + x * 16 + 8) = hi;
-            }
-          }
-        } else {
+        for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
-            const int row = 8 * nb + 2 * i4 + c;
-            if (first + row < a.G) {
-              const long slot = ((long)w * 2 + (seg < f0 ? 0 : 1)) * HG + row;
-              float* pp = a.part + slot * D + g;
+            float mx = fmaxf(sc[nb][c], sc[nb][2 + c]);
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+            const float mn = mx > m[nb][c] + kSlack ? mx : m[nb][c];
+            const float alpha = exp2f(m[nb][c] - mn);
+            m[nb][c] = mn;
+            l[nb][c] *= alpha;
+            const float all = alpha * down;
 #pragma unroll
-              for (int x = 0; x < MT; ++x) {
-                pp[x * 16] = o[nb][x][c] * up[c];
-                pp[x * 16 + 8] = o[nb][x][2 + c] * up[c];
-              }
-              if (g == 0) { a.ml[slot * 2] = m[nb][c]; a.ml[slot * 2 + 1] = l[nb][c]; }
+            for (int x = 0; x < MT; ++x) {
+              o[nb][x][c] *= all;
+              o[nb][x][2 + c] *= all;
             }
+          }
+        vref = vnew;
+        vinv = vnew > 0.f ? __fdiv_rn(1.f, vnew) : 1.f;
+      }
+      const float ratio = va * vinv;
+      const bool faint = ratio < kFaint;                           // (uniform; a NaN magnitude is not)
+      const float pr = faint ? 1.f : ratio;
+      uint32_t pb[NB][2];
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        float pv[4];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) pv[c] = exp2f(sc[nb][c] - m[nb][c & 1]);
+        l[nb][0] += pv[0] + pv[2];
+        l[nb][1] += pv[1] + pv[3];
+        pb[nb][0] = transpose8x8(pack_half2(pv[0] * pr, pv[1] * pr));
+        pb[nb][1] = transpose8x8(pack_half2(pv[2] * pr, pv[3] * pr));
+      }
+      // ---- O^T: dims g and g + 8 of each tile, tokens 4 i4 .. 4 i4 + 3
+      const uint32_t* vw = reinterpret_cast<const uint32_t*>(vt) + g * 4 + i4;
+      if (!faint) {
+#pragma unroll
+        for (int x = 0; x < MT; ++x) {
+          uint32_t f[4];
+          int8x4_to_half(vw[x * 64], f[0], f[2]);
+          int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) mma_f16(o[nb][x], f, pb[nb][0], pb[nb][1]);
+        }
+      } else {
+#pragma unroll
+        for (int x = 0; x < MT; ++x) {
+          uint32_t f[4];
+          int8x4_to_half(vw[x * 64], f[0], f[2]);
+          int8x4_to_half(vw[x * 64 + 32], f[1], f[3]);
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) {
+            float c[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_f16(c, f, pb[nb][0], pb[nb][1]);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[nb][x][k] += c[k] * ratio;
+          }
+        }
+      }
+      __syncwarp();                                                // the stage has been read by all lanes
+      {
+        const int ahead = bi + C::kStages;
+        const int at = __shfl_sync(0xffffffffu, ahead < 32 ? at_c : at_n, ahead & 31);
+        if (t + C::kStages < n) issue(s, at);
+      }
+      if (++s == C::kStages) { s = 0; ph ^= 1; }
+    }
+    // ---- end of this head's tokens, or of this worker's share
+    const int seg = prefix[b] * VH + vh * tb;                  // flat tile the head begins with
+    const bool whole = seg >= f0 && seg + tb <= f1;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb) {
+      __syncwarp();
+      float up[2];
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 4);
+        l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 8);
+        l[nb][c] += __shfl_xor_sync(0xffffffffu, l[nb][c], 16);
+        up[c] = whole ? (l[nb][c] != 0.f ? __fdividef(vref, l[nb][c]) : 0.f) : vref;
+      }
+      if (whole) {
+        // pairs of heads of a dim -> pairs of dims of a head
+        const int head = first + 8 * nb + g;
+        __nv_bfloat16* op = a.out + ((long)b * a.Hq + h0 + head) * D + 2 * i4;
+#pragma unroll
+        for (int x = 0; x < MT; ++x) {
+          const uint32_t lo = transpose8x8(pack_bf16x2(o[nb][x][0] * up[0], o[nb][x][1] * up[1]));
+          const uint32_t hi = transpose8x8(pack_bf16x2(o[nb][x][2] * up[0], o[nb][x][3] * up[1]));
+          if (head < a.G) {
+            *reinterpret_cast<uint32_t*>(op + x * 16) = lo;
+            *reinterpret_cast<uint32_t*>(op + x * 16 + 8) = hi;
+          }
+        }
+      } else {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int row = 8 * nb + 2 * i4 + c;
+          if (first + row < a.G) {
+            const long slot = ((long)w * 2 + (seg < f0 ? 0 : 1)) * HG + row;
+            float* pp = a.part + slot * D + g;
+#pragma unroll
+            for (int x = 0; x < MT; ++x) {
+              pp[x * 16] = o[nb][x][c] * up[c];
+              pp[x * 16 + 8] = o[nb][x][2 + c] * up[c];
+            }
+            if (g == 0) { a.ml[slot * 2] = m[nb][c]; a.ml[slot * 2 + 1] = l[nb][c]; }
           }
         }
       }
     }
-    // ---- next tile: the next token block, KV head or non-empty sequence
-    if (++tile == tb) {
-      tile = 0;
-      fresh = true;
-      if (++vh == VH) {
-        vh = 0;
-        do { ++b; } while (b < a.B && prefix[b + 1] == prefix[b]);
-        if (b < a.B) tb = prefix[b + 1] - prefix[b];
-      }
+    // ---- the next KV head or non-empty sequence
+    tile = 0;
+    if (++vh == VH) {
+      vh = 0;
+      do { ++b; } while (b < a.B && prefix[b + 1] == prefix[b]);
+      if (b < a.B) tb = prefix[b + 1] - prefix[b];
     }
   }
 }
 
-// One block per query head: adds up the partials of a head whose tokens went to several workers, and
-// writes zeros for an empty context.  Its warps take the partials in turn; a lane holds D / 32 dims.
-template <int D, int HG>
+// Adds up the partials of the heads whose tokens went to several workers, and writes zeros for an empty
+// context.  Grid (B Hq, D / SL): a block has SL dims of a head, a group of lanes holds them (four or eight a
+// lane), and the block's groups take the partials in turn; the largest maximum is found first, so that the
+// loads of the sums do not wait for one another.  SL = D for many heads (few blocks and few partials each),
+// 32 for few heads whose tokens went to many workers: 1 sequence of 60000 tokens and one KV head takes 20 us
+// that way, 48 with whole heads a block; 64 sequences of 777 tokens 32 us with whole heads, 41 in slices.
+template <int D, int HG, int SL>
 __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
-  constexpr int E = D / 32;
-  extern __shared__ float smem_f[];                              // [warps][D] + [warps][2]
+  constexpr int LG = SL / 4 < 32 ? SL / 4 : 32;                  // lanes of a group
+  constexpr int NV = SL / 4 / LG;                                // float4s of a lane
+  constexpr int GW = 32 / LG;                                    // groups of a warp
+  __shared__ float s_top[32], s_sum[32];
+  __shared__ float4 s_acc[SL == 32 ? 32 : 8][SL / 4];            // [warps]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   const int b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
   const int h = hq / a.G, hg = hq % a.G, vh = h * a.nblk + hg / HG, row = hg % HG;
@@ -700,71 +697,85 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
     if (b0 + lane < b) before += n;
     if (b0 + lane == b) tb = n;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-    tb += __shfl_xor_sync(0xffffffffu, tb, o);
-  }
-  __nv_bfloat16* op = a.out + ((long)b * a.Hq + hq) * D;
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  tb = __reduce_add_sync(0xffffffffu, tb);
+  __nv_bfloat16* op = a.out + ((long)b * a.Hq + hq) * D + blockIdx.y * SL;
   if (tb == 0) {
-    if (warp == 0)
-      for (int d = lane; d < D; d += 32) op[d] = __float2bfloat16(0.f);
+    for (int d = threadIdx.x; d < SL; d += blockDim.x) op[d] = __float2bfloat16(0.f);
     return;
   }
   const int chunk = chunk_of(a, total * VH), seg = before * VH + vh * tb;
-  const int w0 = seg / chunk, w1 = (seg + tb - 1) / chunk;
-  if (w0 == w1) return;                                          // one worker had it all and wrote it
+  const int w0 = seg / chunk, w1 = (seg + tb - 1) / chunk, pieces = w1 - w0 + 1;
+  if (pieces == 1) return;                                       // one worker had it all and wrote it
+  auto slot_of = [&](int i) { return ((long)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * HG + row; };
   float M = -INFINITY;
-  float acc[E], L = 0.f;
-#pragma unroll
-  for (int e = 0; e < E; ++e) acc[e] = 0.f;
-#pragma unroll 4
-  for (int x = w0 + warp; x <= w1; x += warps) {
-    const long slot = ((long)x * 2 + (x == w0 ? 1 : 0)) * HG + row;
-    const float ms = a.ml[slot * 2], ls = a.ml[slot * 2 + 1];
-    float v[E];
-    const float* pp = a.part + slot * D + lane * E;
-#pragma unroll
-    for (int e = 0; e < E; e += 2) {
-      const float2 t = *reinterpret_cast<const float2*>(pp + e);
-      v[e] = t.x; v[e + 1] = t.y;
-    }
-    const float mn = fmaxf(M, ms), base = mn == -INFINITY ? 0.f : mn;
-    const float fa = exp2f(M - base), fb = exp2f(ms - base);
-    L = L * fa + ls * fb;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = acc[e] * fa + v[e] * fb;
-    M = mn;
-  }
+  for (int i = threadIdx.x; i < pieces; i += blockDim.x) M = fmaxf(M, a.ml[slot_of(i) * 2]);
+  M = warp_max(M);
   if (warps > 1) {
-    float* so = smem_f;
-    float* sm = smem_f + warps * D;
+    if (lane == 0) s_top[warp] = M;
+    __syncthreads();
+    M = warp_max(lane < warps ? s_top[lane] : -INFINITY);
+  }
+  const int sub = lane % LG, group = warp * GW + lane / LG, groups = warps * GW;
+  float4 acc[NV];
 #pragma unroll
-    for (int e = 0; e < E; ++e) so[warp * D + lane * E + e] = acc[e];
-    if (lane == 0) { sm[2 * warp] = M; sm[2 * warp + 1] = L; }
+  for (int k = 0; k < NV; ++k) acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+  float L = 0.f;
+#pragma unroll 4
+  for (int i = group; i < pieces; i += groups) {
+    const long slot = slot_of(i);
+    const float2 ml = *reinterpret_cast<const float2*>(a.ml + slot * 2);
+    const float4* pp = reinterpret_cast<const float4*>(a.part + slot * D + blockIdx.y * SL) + sub;
+    const float f = exp2f(ml.x - M);
+    L += ml.y * f;
+#pragma unroll
+    for (int k = 0; k < NV; ++k) {
+      const float4 v = pp[k * LG];
+      acc[k].x += v.x * f; acc[k].y += v.y * f; acc[k].z += v.z * f; acc[k].w += v.w * f;
+    }
+  }
+  auto add_groups = [&](float4& v) {
+#pragma unroll
+    for (int o = LG; o < 32; o *= 2) {
+      v.x += __shfl_xor_sync(0xffffffffu, v.x, o);
+      v.y += __shfl_xor_sync(0xffffffffu, v.y, o);
+      v.z += __shfl_xor_sync(0xffffffffu, v.z, o);
+      v.w += __shfl_xor_sync(0xffffffffu, v.w, o);
+    }
+  };
+#pragma unroll
+  for (int o = LG; o < 32; o *= 2) L += __shfl_xor_sync(0xffffffffu, L, o);
+#pragma unroll
+  for (int k = 0; k < NV; ++k) add_groups(acc[k]);
+  if (warps > 1) {
+#pragma unroll
+    for (int k = 0; k < NV; ++k)
+      if (lane < LG) s_acc[warp][k * LG + sub] = acc[k];
+    if (lane == 0) s_sum[warp] = L;
     __syncthreads();
     if (warp != 0) return;
-    const float mw = lane < warps ? sm[2 * lane] : -INFINITY;
-    M = warp_max(mw);
-    const float base = M == -INFINITY ? 0.f : M;
-    const float f = exp2f(mw - base);
-    L = warp_sum(lane < warps ? sm[2 * lane + 1] * f : 0.f);
+    L = warp_sum(lane < warps ? s_sum[lane] : 0.f);
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = 0.f;
-    for (int x = 0; x < warps; ++x) {
-      const float fx = __shfl_sync(0xffffffffu, f, x);
-#pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += so[x * D + lane * E + e] * fx;
+    for (int k = 0; k < NV; ++k) {
+      acc[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int x = lane / LG; x < warps; x += GW) {
+        const float4 v = s_acc[x][k * LG + sub];
+        acc[k].x += v.x; acc[k].y += v.y; acc[k].z += v.z; acc[k].w += v.w;
+      }
+      add_groups(acc[k]);
     }
   }
   const float inv = L != 0.f ? __fdividef(1.f, L) : 0.f;
 #pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(op + lane * E + e) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
+  for (int k = 0; k < NV; ++k)
+    if (lane < LG)
+      *reinterpret_cast<uint2*>(op + (k * LG + sub) * 4) =
+          make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
 }
 
 template <int D, int HG>
-int launch_attn(AttnArgs& a, int blocks, int merge_warps, cudaStream_t stream) {
+int launch_attn(AttnArgs& a, int blocks, cudaStream_t stream) {
   using C = AttnCfg<D>;
   auto kern = decode_int8_kernel<D, HG / 8>;
   const int smem = C::kRing + kWarps * C::kStages * 8 + 8 + (a.B + 1) * 4;
@@ -778,7 +789,15 @@ int launch_attn(AttnArgs& a, int blocks, int merge_warps, cudaStream_t stream) {
   }
   int rc = axh::launch_chained(kern, dim3(blocks), dim3(kWarps * 32), smem, 1, stream, a);
   if (rc) return rc;
-  return axh::launch_chained(merge_int8_kernel<D, HG>, dim3(a.B * a.Hq), dim3(32 * merge_warps), merge_warps * (D + 2) * 4, 1, stream, a);
+  // partials of a head, at the most if heads are alike
+  const long heads = (long)a.B * a.Hkv * a.nblk, per = a.workers / heads + 2;
+  int warps = 1;
+  if ((long)a.B * a.Hq >= 4 * axh::sm_count()) {
+    while (warps < 8 && warps * 2 < per) warps *= 2;
+    return axh::launch_chained(merge_int8_kernel<D, HG, D>, dim3(a.B * a.Hq), dim3(32 * warps), 0, 1, stream, a);
+  }
+  while (warps < 32 && warps * 4 < per) warps *= 2;
+  return axh::launch_chained(merge_int8_kernel<D, HG, 32>, dim3(a.B * a.Hq, D / 32), dim3(32 * warps), 0, 1, stream, a);
 }
 
 }  // namespace
@@ -803,24 +822,38 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   return axh::launch_chained(kv_write_int8_kernel<float>, grid, dim3(2 * kHalf), 0, 1, stream, a);
 }
 
-// Workers (warps) the attention kernel runs with: what fills the device, fewer for a small cache.
-static int attn_blocks(int B, int VH, int D, int HG, int max_pages, int P, int min_chunk) {
-  const long tiles = (long)B * VH * ((long)max_pages * P / kTile);
-  const long want = (tiles + (long)min_chunk * kWarps - 1) / ((long)min_chunk * kWarps);
-  const long most = (long)axh::sm_count() * (HG == 16 || D == 256 ? 2 : 4);
-  const long few = (tiles + min_chunk - 1) / min_chunk;           // one worker a block while that spreads them further
-  const long n = want < axh::sm_count() ? (few < axh::sm_count() ? few : axh::sm_count()) : want;
-  return (int)(n < most ? (n > 0 ? n : 1) : most);
+// How the attention kernel is launched for a cache of this capacity.
+struct AttnShape { int HG, nblk, min_chunk, blocks; };
+static AttnShape attn_shape(int B, int Hq, int Hkv, int D, int max_pages, int P) {
+  AttnShape r;
+  const int G = Hq / Hkv;
+  r.HG = G <= 8 ? 8 : 16;
+  r.nblk = (G + r.HG - 1) / r.HG;
+  const long per_head = (long)max_pages * P / kTile, tiles = (long)B * Hkv * r.nblk * per_head;
+  const long most = (long)axh::sm_count() * (r.HG == 16 || D == 256 ? 2 : 4);
+  // The fewest tiles a worker takes: every tile in turn costs it about 0.45 us, every worker a partial that the
+  // merge has to read, so a share grows with the root of the context (1 sequence of 4096 tokens, 8 KV
+  // heads: 13.8 us with shares of one tile, 12.1 with four; 100 tokens: 7.3 and 10.9).
+  long chunk = 1;
+  while ((chunk + 1) * (chunk + 1) * 16 < per_head) ++chunk;
+  r.min_chunk = (int)(chunk < 64 ? chunk : 64);
+  // Blocks whose warps all have a share; where that leaves SMs without a block, fewer warps a block.
+  const long even = (tiles + most * kWarps - 1) / (most * kWarps);
+  if (even > chunk) chunk = even;
+  long n = (tiles + chunk * kWarps - 1) / (chunk * kWarps);
+  if (n < axh::sm_count()) {
+    n = (tiles + chunk - 1) / chunk;
+    if (n > axh::sm_count()) n = axh::sm_count();
+  }
+  r.blocks = (int)(n < 1 ? 1 : (n < most ? n : most));
+  return r;
 }
-
-constexpr int kMinChunk = 4;
 
 // Floats of workspace that ax_decode_int8 needs (0: an argument it refuses).
 AX_API long ax_decode_int8_workspace(int B, int Hq, int Hkv, int D, int max_pages, int P) {
   if (Hkv <= 0 || Hq % Hkv || P <= 0) return 0;
-  const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
-  const long workers = (long)attn_blocks(B, Hkv * nblk, D, HG, max_pages, P, kMinChunk) * kWarps;
-  return workers * 2 * HG * (D + 2);
+  const AttnShape r = attn_shape(B, Hq, Hkv, D, max_pages, P);
+  return (long)r.blocks * kWarps * 2 * r.HG * (D + 2);
 }
 
 // out[B, Hq, D] = attention of q[B, Hq, D] (bf16, contiguous) over the first ctx[b] tokens of each sequence.
@@ -832,17 +865,13 @@ AX_API int ax_decode_int8(const void* q, const int8_t* kc, const int8_t* vc, con
   if (B <= 0) return 0;
   if (Hkv <= 0 || Hq % Hkv || P <= 0 || P % 16 || B > 8192 || (long)B * Hq > 0x7fffffffL) return -1;
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)workspace) & 15) return -2;
-  const int G = Hq / Hkv, HG = G <= 8 ? 8 : 16, nblk = (G + HG - 1) / HG;
-  if ((long)B * Hkv * nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv * (P / kTile) > 0x7fffffffL) return -3;
-  const int blocks = attn_blocks(B, Hkv * nblk, D, HG, max_pages, P, kMinChunk);
-  const int workers = blocks * kWarps;
+  const AttnShape r = attn_shape(B, Hq, Hkv, D, max_pages, P);
+  const int HG = r.HG, blocks = r.blocks, workers = blocks * kWarps;
+  if ((long)B * Hkv * r.nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv * (P / kTile) > 0x7fffffffL) return -3;
   AttnArgs a{(const __nv_bfloat16*)q, kc, vc, ka, va, table, ctx, (__nv_bfloat16*)out, workspace, workspace + (long)workers * 2 * HG * D,
-             B, Hq, Hkv, G, nblk, P, max_pages, num_pages, kMinChunk, workers, scale * 1.4426950408889634f / 127.f, status};
-  // partials per head: many when few heads share all workers
-  const long heads = (long)B * Hkv * nblk, per = workers / (heads > 0 ? heads : 1) + 1;
-  const int mw = per <= 2 ? 1 : (per <= 8 ? 4 : (per <= 32 ? 8 : 16));
+             B, Hq, Hkv, Hq / Hkv, r.nblk, P, max_pages, num_pages, r.min_chunk, workers, scale * 1.4426950408889634f / 127.f, status};
 #define AX_ATTN(DD)                                                      \
-  return HG == 8 ? launch_attn<DD, 8>(a, blocks, mw, stream) : launch_attn<DD, 16>(a, blocks, mw, stream)
+  return HG == 8 ? launch_attn<DD, 8>(a, blocks, stream) : launch_attn<DD, 16>(a, blocks, stream)
   switch (D) {
     case 64: AX_ATTN(64);
     case 128: AX_ATTN(128);
