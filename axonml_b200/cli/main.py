@@ -706,8 +706,11 @@ def cmd_serve(a):
     engine = None
     if a.gguf:
         from ..server import LLMEngine, QuantizedLlama
-        engine = LLMEngine(QuantizedLlama.from_gguf(a.gguf, device="cuda" if torch.cuda.is_available() else "cpu"),
-                           max_batch=a.max_batch, max_context=a.max_context)
+        model = QuantizedLlama.from_gguf(a.gguf, device="cuda" if torch.cuda.is_available() else "cpu")
+        if a.weights == "int8":
+            model.to_int8()
+        engine = LLMEngine(model, max_batch=a.max_batch, max_context=a.max_context,
+                           kv_dtype=torch.int8 if a.kv_cache == "int8" else torch.bfloat16)
         engine.warmup()
     inf = InferenceServer()
     specs = list(a.model or [])
@@ -902,6 +905,8 @@ def build_parser() -> argparse.ArgumentParser:
     p.add_argument("-p", "--port", type=int, default=3021)
     p.add_argument("--model", action="append", help="name=path of a StateDict model"); p.add_argument("--gguf")
     p.add_argument("--max-batch", "--max-batch-size", type=int, default=64, dest="max_batch"); p.add_argument("--max-context", type=int, default=1024)
+    p.add_argument("--kv-cache", choices=("bf16", "int8"), default="bf16", help="type the engine's K/V cache is kept in")
+    p.add_argument("--weights", choices=("keep", "int8"), default="keep", help="int8: projections with one scale per channel")
     p.add_argument("--workers", type=int, default=4, help="accepted for compatibility: requests are served by one thread per connection")
     p.add_argument("--batch", action="store_true", help="accepted for compatibility: the LLM engine always batches")
     p.add_argument("--timeout", type=int, default=30000, help="per-request timeout in ms")

@@ -30,7 +30,10 @@ class Request:
 
 class LLMEngine:
     def __init__(self, model, max_batch: int = 64, max_context: int = 1024, page_size: int = 16,
-                 num_pages: int | None = None):
+                 num_pages: int | None = None, kv_dtype: torch.dtype = torch.bfloat16):
+        """``kv_dtype``: bf16, or int8 for a cache of half the size (pages of a multiple of 16 tokens)."""
+        if kv_dtype not in (torch.bfloat16, torch.int8):
+            raise ValueError(f"kv_dtype must be bf16 or int8, not {kv_dtype}")
         self.model, self.max_batch = model, max_batch
         if hasattr(model, "optimize_layout"):
             model.optimize_layout()
@@ -38,7 +41,7 @@ class LLMEngine:
         pages_per_seq = (max_context + page_size - 1) // page_size
         num_pages = num_pages or max_batch * pages_per_seq
         self.cache = PagedKVCache(cfg.num_hidden_layers, num_pages, page_size, model.hkv, model.hd, max_batch,
-                                  pages_per_seq, model.device)
+                                  pages_per_seq, model.device, dtype=kv_dtype)
         self.waiting: list[Request] = []
         self.running: list[Request] = []
         self.finished: list[Request] = []

@@ -3,9 +3,11 @@ paged KV cache, tensor parallel over the process group (heads and FFN columns sp
 vocabulary-parallel head).  Weights come from a GGUF file or are drawn N(0, 0.02) and quantised on
 the GPU (``from_random``).
 
-Every projection is the fused dequantising matmul (``ops.quant.qlinear``); prefill attention is
-the flash kernel, decode attention reads the paged cache; the two all-reduces per layer use the
-fused peer-memory all-reduce kernel when symmetric memory is available, NCCL otherwise."""
+Every projection is the fused dequantising matmul (``ops.quant.qlinear``) or, after ``to_int8``, the
+int8 product of int8 activations (``ops.int8``: norm and SwiGLU write the rows it reads); prefill
+attention is the flash kernel, decode attention reads the paged cache (bf16 or int8); the two
+all-reduces per layer use the fused peer-memory all-reduce kernel when symmetric memory is
+available, NCCL otherwise."""
 from __future__ import annotations
 
 import math
@@ -14,9 +16,9 @@ import torch
 
 from ..llm.config import LLaMAConfig
 from ..ops import elementwise as E
+from ..ops import int8 as I8
 from ..ops import misc as Mi
 from ..ops import norm as Nm
-from ..ops import paged
 from ..ops.attention import sdpa
 from ..ops.quant import qlinear
 from ..quant.quantize import dequantize_tensor, quantize_tensor
@@ -140,6 +142,8 @@ class QuantizedLlama:
     def to_gguf(self, path) -> None:
         """Writes this rank's weights as a GGUF file (single-rank models are complete checkpoints)."""
         from ..quant.gguf import write_gguf
+        if self.int8_weights():
+            raise ValueError("int8 projections (one scale per channel) have no GGUF type: write the model before to_int8()")
         c, hd = self.cfg, self.hd
         t, nq, nk = {}, self.hq * hd, self.hkv * hd
 
@@ -167,7 +171,7 @@ class QuantizedLlama:
         if self.device.type != "cuda":
             return self
         from ..ops.quant import tile_weight
-        ok = lambda q: q.layout == "ggml" and q.quant_type in (QuantType.Q4_K, QuantType.Q8_0) and q.shape[1] % 256 == 0
+        ok = lambda q: isinstance(q, QuantizedTensor) and q.layout == "ggml" and q.quant_type in (QuantType.Q4_K, QuantType.Q8_0) and q.shape[1] % 256 == 0
         for L in self.layers:
             for name in ("wqkv", "wo", "wgu", "wdown"):
                 q = getattr(L, name)
@@ -176,6 +180,24 @@ class QuantizedLlama:
         if ok(self.head):
             self.head = tile_weight(self.head)
         return self
+
+    def to_int8(self) -> "QuantizedLlama":
+        """Converts the projections to int8 with one scale per output channel (``ops.int8.Int8Weight``).
+        Prefill and decode then run them as int8 products of int8 activations with one scale per token:
+        twice the bytes of Q4_K to read when decoding a few sequences, twice the tensor rate of the
+        dequantised product in prefill and large batches.  Embedding and head keep their type."""
+        from ..ops.quant import untile_weight
+        for L in self.layers:
+            for name in ("wqkv", "wo", "wgu", "wdown"):
+                w = getattr(L, name)
+                if not isinstance(w, I8.Int8Weight):
+                    if w.layout == "tile128":
+                        w = untile_weight(w)
+                    setattr(L, name, I8.Int8Weight.from_dense(dequantize_tensor(w)))
+        return self
+
+    def int8_weights(self) -> bool:
+        return bool(self.layers) and isinstance(self.layers[0].wqkv, I8.Int8Weight)
 
     def weight_bytes(self) -> int:
         n = self.embed.size_bytes() + self.head.size_bytes()
@@ -262,28 +284,52 @@ class QuantizedLlama:
         x = self._embed(ids).view(B * S, -1)
         seq = torch.tensor(slots, dtype=torch.int32, device=self.device).repeat_interleave(S)
         pos = torch.arange(S, dtype=torch.int32, device=self.device).repeat(B)
+        table, starts, rows = cache.block_table, None, seq
+        if cache.int8:
+            table = cache.block_table[torch.tensor(slots, dtype=torch.long, device=self.device)]
+            starts = torch.zeros(B, dtype=torch.int32, device=self.device)
         nq, nk = self.hq * self.hd, self.hkv * self.hd
+        int8, eps = self.int8_weights(), self.cfg.rms_norm_eps
+        d = None
         for li, L in enumerate(self.layers):
-            h = Nm.rms_norm(x, L.attn_norm, self.cfg.rms_norm_eps)
-            qkv = qlinear(h, L.wqkv).view(B * S, self.hq + 2 * self.hkv, self.hd)
+            if int8:
+                h, x = self._norm_rows(x if d is None else d, L.attn_norm, None if d is None else x)
+                qkv = self._rows_linear(h, L.wqkv)
+            else:
+                qkv = qlinear(Nm.rms_norm(x, L.attn_norm, eps), L.wqkv)
+            qkv = qkv.view(B * S, self.hq + 2 * self.hkv, self.hd)
             qkv = Mi.rope_positions(qkv, self.cos, self.sin, pos, rot_heads=self.hq + self.hkv)
             q, k, v = qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv], qkv[:, self.hq + self.hkv:]
-            paged.kv_write(k, v, cache.k[li], cache.v[li], cache.block_table, seq, pos, cache.page_size)
+            cache.write(li, k, v, table, starts, rows, pos)
             a = sdpa(q.reshape(B, S, self.hq, self.hd), k.reshape(B, S, self.hkv, self.hd),
                      v.reshape(B, S, self.hkv, self.hd), causal=True)
-            o = self._all_reduce(qlinear(a.reshape(B * S, nq), L.wo))
-            x = x + o
-            h = Nm.rms_norm(x, L.ffn_norm, self.cfg.rms_norm_eps)
-            d = self._all_reduce(qlinear(E.swiglu(qlinear(h, L.wgu)), L.wdown))
+            if int8:
+                o = self._all_reduce(L.wo.linear(a.reshape(B * S, nq)))
+                h, x = self._norm_rows(o, L.ffn_norm, x)
+                d = self._all_reduce(self._rows_linear(I8.swiglu_int8(self._rows_linear(h, L.wgu)), L.wdown))
+            else:
+                o = self._all_reduce(qlinear(a.reshape(B * S, nq), L.wo))
+                x = x + o
+                h = Nm.rms_norm(x, L.ffn_norm, eps)
+                x = x + self._all_reduce(qlinear(E.swiglu(qlinear(h, L.wgu)), L.wdown))
+        if int8 and d is not None:
             x = x + d
         return x.view(B, S, -1)[:, -1]
+
+    def _norm_rows(self, x, weight, residual=None):
+        """RMSNorm of ``x (+ residual)`` to int8 rows, and the stream that was normalised."""
+        got = I8.rms_norm_int8(x, weight, self.cfg.rms_norm_eps, residual=residual)
+        return (got[0], got[1]), (x if residual is None else got[2])
+
+    def _rows_linear(self, rows, w) -> torch.Tensor:
+        return I8.int8_linear(rows[0], rows[1], w.q, w.scale)
 
     def _fused_decode_ok(self, B: int, cache) -> bool:
         """Batches of up to four rows on the matrix-vector kernels: every producer writes int8
         activations itself and RoPE + KV write are one launch (``ops/decode.py``)."""
         import os
         from ..ops import decode as Dc
-        if os.environ.get("AXONML_DECODE_FUSED", "1") == "0" or self.hd != 128 or not self.layers:
+        if os.environ.get("AXONML_DECODE_FUSED", "1") == "0" or self.hd != 128 or not self.layers or cache.int8 or self.int8_weights():
             return False
         from .. import _native as N
         L = self.layers[0]
@@ -329,18 +375,30 @@ class QuantizedLlama:
         table = cache.block_table[slots_t.long()]
         seq_local = torch.arange(B, dtype=torch.int32, device=self.device)
         nq = self.hq * self.hd
-        h = Nm.rms_norm(x, self.layers[0].attn_norm, self.cfg.rms_norm_eps)
+        int8, eps = self.int8_weights(), self.cfg.rms_norm_eps
+        if int8:
+            h, x = self._norm_rows(x, self.layers[0].attn_norm)
+        else:
+            h = Nm.rms_norm(x, self.layers[0].attn_norm, eps)
         for li, L in enumerate(self.layers):
-            qkv = qlinear(h, L.wqkv).view(B, self.hq + 2 * self.hkv, self.hd)
+            qkv = (self._rows_linear(h, L.wqkv) if int8 else qlinear(h, L.wqkv)).view(B, self.hq + 2 * self.hkv, self.hd)
             qkv = Mi.rope_positions(qkv, self.cos, self.sin, positions, rot_heads=self.hq + self.hkv)
             q, k, v = qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv], qkv[:, self.hq + self.hkv:]
-            paged.kv_write(k, v, cache.k[li], cache.v[li], table, seq_local, positions, cache.page_size)
-            a = paged.decode_attention(q.contiguous(), cache.k[li], cache.v[li], table, ctx, cache.page_size)
-            o = self._all_reduce(qlinear(a.reshape(B, nq), L.wo))
-            h, x = Nm.rms_norm(o, L.ffn_norm, self.cfg.rms_norm_eps, residual=x)     # x += o, fused
-            d = self._all_reduce(qlinear(E.swiglu(qlinear(h, L.wgu)), L.wdown))
-            if li + 1 < len(self.layers):
-                h, x = Nm.rms_norm(d, self.layers[li + 1].attn_norm, self.cfg.rms_norm_eps, residual=x)
+            cache.write(li, k, v, table, positions, seq_local, positions)
+            a = cache.attend(li, q.contiguous(), table, ctx)
+            nxt = self.layers[li + 1].attn_norm if li + 1 < len(self.layers) else None
+            if int8:
+                o = self._all_reduce(L.wo.linear(a.reshape(B, nq)))
+                h, x = self._norm_rows(o, L.ffn_norm, x)                             # x += o, fused
+                d = self._all_reduce(self._rows_linear(I8.swiglu_int8(self._rows_linear(h, L.wgu)), L.wdown))
+                if nxt is not None:
+                    h, x = self._norm_rows(d, nxt, x)
             else:
+                o = self._all_reduce(qlinear(a.reshape(B, nq), L.wo))
+                h, x = Nm.rms_norm(o, L.ffn_norm, eps, residual=x)                   # x += o, fused
+                d = self._all_reduce(qlinear(E.swiglu(qlinear(h, L.wgu)), L.wdown))
+                if nxt is not None:
+                    h, x = Nm.rms_norm(d, nxt, eps, residual=x)
+            if nxt is None:
                 x = x + d
         return x

@@ -84,3 +84,73 @@ def attention(q, k_rows, v_rows_, ka, va, table, ctx, scale):
 
 def default_scale(D):
     return 1.0 / math.sqrt(D)
+
+
+class Recorder:
+    """Records every int8 operator call of a run, inputs and outputs, and checks each against the definition in 64 bits.
+    (Whole models are not compared with unquantised ones: a rounding of one percent of a score of eighty is a factor of two in
+    its weight, so nothing bounds that distance.)"""
+
+    def __init__(self, monkeypatch):
+        from axonml_b200.ops import int8, paged
+        self.calls = []
+        for mod, name in ((int8, "rms_norm_int8"), (int8, "swiglu_int8"), (int8, "quantize_int8"), (int8, "int8_linear"),
+                          (paged, "kv_write_int8"), (paged, "decode_attention_int8")):
+            monkeypatch.setattr(mod, name, self._wrap(name, getattr(mod, name)))
+
+    def _wrap(self, name, fn):
+        def call(*args, **kw):
+            copy = [a.clone() if torch.is_tensor(a) else a for a in args]
+            got = fn(*args, **kw)
+            after = [a.clone() for a in args[2:6]] if name == "kv_write_int8" else got
+            self.calls.append((name, copy, dict(kw), after))
+            return got
+        return call
+
+    def names(self):
+        return [c[0] for c in self.calls]
+
+    def check(self):
+        for name, a, kw, got in self.calls:
+            getattr(self, "_" + name)(a, kw, got)
+
+    @staticmethod
+    def _rows(q, s, y, off):
+        # half a step, and what the value itself and its scale are off: `off` of the row's largest value
+        assert ((q.double() * s.double()[..., None] - y).abs() <= s.double()[..., None] * (0.5 + 127 * 2 * off)).all()
+        assert ((s.double() - y.abs().amax(-1) / 127).abs() <= off * s.double()).all()
+
+    def _rms_norm_int8(self, a, kw, got):
+        x, w, eps = a[0], a[1], a[2]
+        h = x if kw.get("residual") is None else x + kw["residual"]
+        if kw.get("residual") is not None:
+            assert torch.equal(got[2], h)
+        d = h.double()
+        # the sum of squares: at most D / 256 + 12 roundings in any order, halved by the root; eight more elsewhere
+        off = (d.shape[-1] / 512 + 14) * 2.0 ** -24
+        self._rows(got[0], got[1], d * torch.rsqrt(d.pow(2).mean(-1, keepdim=True) + eps) * w.double(), off)
+
+    def _swiglu_int8(self, a, kw, got):
+        g, u = a[0].double().chunk(2, -1)
+        # exp's two steps and its argument's rounding (below 2^5 here, times log2(e)), reciprocal's two, two products
+        self._rows(got[0], got[1], g * torch.sigmoid(g) * u, (2 * 2 + 32 * 1.45 + 2 * 2 + 4) * 2.0 ** -24)
+
+    def _quantize_int8(self, a, kw, got):
+        self._rows(got[0], got[1], a[0].double(), 2 * 2.0 ** -24)
+
+    def _int8_linear(self, a, kw, got):
+        want = (a[0].double() @ a[2].double().t()) * a[1].double()[:, None] * a[3].double()
+        assert got.dtype == torch.bfloat16 and ((got.double() - want).abs() <= (2.0 ** -8 + 4 * 2.0 ** -24) * want.abs()).all()
+
+    def _kv_write_int8(self, a, kw, got):
+        k, v, kc, vc, ka, va, table, starts = a[:8]
+        n = k.shape[0] // table.shape[0]
+        cu = [n * i for i in range(table.shape[0] + 1)]
+        for x, rows, amax, c, m in ((k, kc, ka, got[0], got[2]), (v, v_rows(vc), va, v_rows(got[1]), got[3])):
+            want = write(rows.double(), amax.double(), x, table.tolist(), starts.tolist(), cu)
+            assert torch.equal(c.double(), want[0]) and torch.equal(m.double(), want[1])
+
+    def _decode_attention_int8(self, a, kw, got):
+        q, kc, vc, ka, va, table, ctx = a[:7]
+        want, off = attention(q, kc, v_rows(vc), ka, va, table.tolist(), ctx.tolist(), default_scale(q.shape[-1]))
+        assert ((got.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()

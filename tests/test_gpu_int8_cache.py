@@ -190,3 +190,40 @@ def test_write_then_attend_in_a_graph_and_on_another_stream(kernel_status):
         assert torch.equal(out, want)
     for a, b in zip(caches, eager):
         assert torch.equal(a, b)
+
+
+def _gpu_model(**kw):
+    from axonml_b200.llm import LLaMAConfig
+    from axonml_b200.quant import QuantType
+    from axonml_b200.server import QuantizedLlama
+    cfg = LLaMAConfig(vocab_size=20000, hidden_size=1024, intermediate_size=2048, num_hidden_layers=2, num_attention_heads=8,
+                      num_key_value_heads=4, max_position_embeddings=256)
+    return QuantizedLlama.from_random(cfg, None, device="cuda", std=0.05, proj_type=QuantType.Q4_K, **kw)
+
+
+@pytest.mark.parametrize("weights,kv", [(True, torch.int8), (False, torch.int8), (True, torch.bfloat16)])
+def test_engine_in_eight_bits(weights, kv, kernel_status, monkeypatch):
+    """Every operator call of a prefill and a decode step against 64 bits; decoding with graphs against the same without."""
+    from axonml_b200.server import LLMEngine, PagedKVCache
+    model8 = _gpu_model()
+    prompts = [[(11 * i + j) % 19000 for j in range(20)] for i in range(5)]
+    cache = PagedKVCache(2, 16, 16, model8.hkv, model8.hd, 5, 3, model8.device, dtype=kv)
+    if weights:
+        model8.to_int8()
+    slots = [cache.allocate_seq() for _ in prompts]
+    for s in slots:
+        cache.reserve(s, 21)
+    with monkeypatch.context() as mp, torch.no_grad():
+        rec = R.Recorder(mp)
+        model8.prefill(torch.tensor(prompts, device="cuda"), cache, slots)
+        model8.decode(torch.arange(5, device="cuda"), cache, torch.tensor(slots, dtype=torch.int32, device="cuda"),
+                      torch.full((5,), 20, dtype=torch.int32, device="cuda"))
+    assert len(rec.calls) == 2 * 2 * ((8 if weights else 0) + (1 if kv == torch.int8 else 0)) + (2 if kv == torch.int8 else 0)
+    rec.check()
+    monkeypatch.setenv("AXONML_DECODE_GRAPHS", "1")
+    a = LLMEngine(model8, max_batch=5, max_context=64, page_size=16, kv_dtype=kv).generate(prompts, 24)
+    monkeypatch.setenv("AXONML_DECODE_GRAPHS", "0")
+    b = LLMEngine(model8, max_batch=5, max_context=64, page_size=16, kv_dtype=kv).generate(prompts, 24)
+    assert all(len(x) == 24 for x in a + b)
+    if weights:                                           # the Q4_K product adds split sums in no fixed order, the int8 one is exact
+        assert a == b
