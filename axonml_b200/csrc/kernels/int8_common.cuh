@@ -3,9 +3,10 @@
 //
 //   q = rint(127 t / a),  a = the group's largest magnitude,  value = q a / 127
 //
-// Products of two bf16 values are exact in fp32, and so is that times 127 (8 + 8 + 7 bits), so the
-// correctly rounded quotient decides every rounding as the real number would, ties included: the
-// result does not depend on the order in which anything was summed.
+// The quotient is formed from 127 / a in two floats, so that it is the real one rounded once to fp32: a quotient
+// that lies on a border between two steps (a value of exactly half the largest is 63.5 steps, and bf16 values
+// are that often) is that border exactly and goes to the even step.  Products of two bf16 values are exact in
+// fp32, so no rounding depends on the order in which anything was summed.
 #pragma once
 #include "common.cuh"
 
@@ -28,64 +29,40 @@ __device__ __forceinline__ float amax_nan(float a, float x) {
   return r;
 }
 
-// What a group's largest magnitude means for its values.
+// What a group's largest magnitude means for its values: t -> t (n / a), n = 127 for values, the old
+// magnitude for steps that move to a larger one.
 struct Int8Grid {
-  float amax, inv;     // inv = 127 / amax
-  bool live;           // false: the magnitude is zero, below the normal numbers, or not finite; all steps are 0
-  bool exact;          // the inverse overflows: divide for every value
+  float hi, lo;        // n / a as a sum of two floats; 0 for a group whose steps are all 0
 };
-__device__ __forceinline__ Int8Grid int8_grid(uint32_t top) {
-  Int8Grid g;
-  g.live = top >= 0x00800000u && top < 0x7f800000u;
-  g.amax = __uint_as_float(top);
-  g.inv = g.live ? __fdiv_rn(127.f, g.amax) : 0.f;
-  g.exact = !(g.inv < 3.0e38f);
+constexpr uint32_t kTinyBits = 7u << 23;   // 2^-120: below it a group counts as zero (127 / a would overflow)
+__device__ __forceinline__ Int8Grid int8_grid(uint32_t top, float n = 127.f) {
+  Int8Grid g{0.f, 0.f};
+  if (top >= kTinyBits && top < 0x7f800000u) {
+    const float a = __uint_as_float(top);
+    g.hi = __fdiv_rn(n, a);
+    g.lo = __fdividef(__fmaf_rn(-g.hi, a, n), a);
+  }
   return g;
 }
 
 // Adding 1.5 * 2^23 rounds a number below 2^22 to the nearest whole one (ties to even) and leaves that number,
 // in two's complement, in the low bits of the sum: no conversion instruction, which the SM has at a
 // sixteenth of the rate of additions.
-constexpr float kRound = 12582912.f;
-
-// t * inv is off by at most two roundings of a number <= 127, i.e. by 1.6e-5: a value further than 3e-5 from
-// the border between two steps is on its side already.  Only the others (one in 16000) take the division.
-constexpr float kBorder = 0.5f - 3.0e-5f;
-
-__device__ __forceinline__ uint32_t int8_exact_bits(float t, float amax) {
-  return __float_as_uint(__fadd_rn(__fdiv_rn(__fmul_rn(t, 127.f), amax), kRound));
+__device__ __forceinline__ uint32_t int8_bits(float t, const Int8Grid& g) {
+  return __float_as_uint(__fadd_rn(__fmaf_rn(t, g.hi, __fmul_rn(t, g.lo)), 12582912.f));
 }
 
 __device__ __forceinline__ uint32_t pack_low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
 }
 
-// Steps of N values (N a multiple of 4) as packed bytes.
-template <int N>
-__device__ __forceinline__ void int8_steps(const float (&t)[N], const Int8Grid& g, uint32_t (&packed)[N / 4]) {
-  uint32_t b[N];
-  float worst = g.exact ? 1.f : 0.f;
+// Steps of eight values as packed bytes.  (A value that is not finite makes its group's grid zero and its own
+// byte something; the group's magnitude says that none of them mean anything.)
+__device__ __forceinline__ uint2 int8_steps(const float (&t)[8], const Int8Grid& g) {
+  uint32_t b[8];
 #pragma unroll
-  for (int j = 0; j < N; ++j) {
-    const float f = t[j] * g.inv;
-    const float r = __fadd_rn(f, kRound);
-    worst = fmaxf(worst, fabsf(f - __fadd_rn(r, -kRound)));
-    b[j] = __float_as_uint(r);
-  }
-  if (worst > kBorder) {
-#pragma unroll
-    for (int j = 0; j < N; ++j) b[j] = int8_exact_bits(t[j], g.amax);
-  }
-#pragma unroll
-  for (int j = 0; j < N; j += 4) packed[j / 4] = g.live ? pack_low_bytes(b[j], b[j + 1], b[j + 2], b[j + 3]) : 0u;
-}
-
-// One value.
-__device__ __forceinline__ int8_t int8_step(float t, const Int8Grid& g) {
-  const float f = t * g.inv;
-  float r = __fadd_rn(f, kRound);
-  if (fabsf(f - __fadd_rn(r, -kRound)) > kBorder || g.exact) r = __uint_as_float(int8_exact_bits(t, g.amax));
-  return g.live ? (int8_t)(__float_as_uint(r) & 255u) : (int8_t)0;
+  for (int j = 0; j < 8; ++j) b[j] = int8_bits(t[j], g);
+  return make_uint2(pack_low_bytes(b[0], b[1], b[2], b[3]), pack_low_bytes(b[4], b[5], b[6], b[7]));
 }
 
 // Eight consecutive values, as they lie in memory and as numbers.

@@ -6,10 +6,11 @@
 //   a = max |y| over the row,  q = rint(127 y / a),  scale = a / 127
 //
 // The norm's 1 / sqrt(...) is one number for the row, so it cancels in q: q = rint(127 t / max |t|),
-// and only the scale carries it.  One block per row; the row is read once and stays in registers
-// between the reduction (sum of squares and largest magnitude together) and the rounding; rows too
-// wide for that are read twice, the second time from L2.  The kernels are bound by the bytes of
-// x, r, h and q.
+// and only the scale carries it.  A block takes a row at a time; the row is read once and stays in registers
+// between the reduction (sum of squares and largest magnitude together) and the rounding, and the block's
+// next row is requested before that reduction, so that its loads travel while this row is rounded.  Rows too
+// wide for registers are read twice, the second time from L2.  The kernels are bound by the bytes of x, r, h
+// and q: norm of 8192 x 4096 bf16 with a residual @@N us, SwiGLU of 4096 x 11008 @@S us.
 #include "int8_common.cuh"
 
 namespace {
@@ -37,185 +38,230 @@ struct RowArgs {
   float eps;
 };
 
-// Sum and largest bits over the block; every thread gets both.
-__device__ __forceinline__ void block_stats(float& sum, uint32_t& top) {
-  __shared__ float s_sum[32];
-  __shared__ uint32_t s_top[32];
+// Sum (where SUM) and largest bits over the block; every thread gets both.  `turn` alternates between two sets of
+// shared words, so that one barrier a row is enough.
+template <bool SUM>
+__device__ __forceinline__ void block_stats(float& sum, uint32_t& top, int turn) {
+  __shared__ float s_sum[2][32];
+  __shared__ uint32_t s_top[2][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  sum = warp_sum(sum);
+  if (SUM) sum = warp_sum(sum);
   top = __reduce_max_sync(0xffffffffu, top);
   if (warps == 1) return;
-  if (lane == 0) { s_sum[warp] = sum; s_top[warp] = top; }
+  if (lane == 0) { s_sum[turn][warp] = sum; s_top[turn][warp] = top; }
   __syncthreads();
-  sum = warp_sum(lane < warps ? s_sum[lane] : 0.f);
-  top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[lane] : 0u);
+  if (SUM) sum = warp_sum(lane < warps ? s_sum[turn][lane] : 0.f);
+  top = __reduce_max_sync(0xffffffffu, lane < warps ? s_top[turn][lane] : 0u);
 }
 
-// KEEP: VPT groups of eight values stay in registers (D <= VPT * 8 * threads).  Otherwise the row
-// is walked twice.  VEC: rows and D allow 16-byte accesses; otherwise a thread's values lie
-// blockDim apart, so that a warp's accesses are still contiguous.  All loads of a walk come before its
-// stores of h: the compiler may not move a load across a store that could alias it.
-template <int MODE, typename T, typename WT, int VPT, bool KEEP, bool VEC>
-__global__ void __launch_bounds__(VPT == 4 ? 512 : 1024) int8_rows_kernel(const RowArgs a) {
-  const long row = blockIdx.x;
-  const T* x = (const T*)a.x + row * a.xs;
-  const bool res = MODE == kNorm && a.res != nullptr;
-  const T* r = res ? (const T*)a.res + row * a.rs : nullptr;
-  T* h = res ? (T*)a.h + row * a.hs : nullptr;
-  const WT* w = (const WT*)a.w;
-  int8_t* q = a.q + row * a.qs;
-  const int tid = threadIdx.x, n = blockDim.x;
-  constexpr int W = VEC ? 8 : 1;                 // values of an access
-  constexpr int S = VEC ? VPT : VPT * 8;         // accesses of a thread (KEEP)
-  float t[VPT][8];
-  float sum = 0.f, most = 0.f;
-  chain_ready();
-  chain_wait();
+template <int MODE>
+__device__ __forceinline__ void write_scale(const RowArgs& a, long row, float sum, uint32_t top) {
+  const float rstd = MODE == kNorm ? __frsqrt_rn(__fdiv_rn(sum, (float)a.D) + a.eps) : 1.f;
+  a.scale[row] = __fdiv_rn(__fmul_rn(top < kTinyBits ? 0.f : __uint_as_float(top), rstd), 127.f);
+}
 
-  // values of accesses [i0, i0 + S) of this thread into t; `out` says whether h is written
-  auto walk = [&](int i0, bool out) {
-    if constexpr (VEC) {
-      Raw8<T> xv[VPT], second[MODE == kPlain ? 1 : VPT];
+// Rows and D allow 16-byte accesses, and VPT groups of eight values a thread cover a row.
+template <int MODE, bool RES, typename T, typename WT, int VPT>
+__global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSwiglu ? 2 : 1) int8_rows_kernel(const RowArgs a, int rows) {
+  const WT* w = (const WT*)a.w;
+  const int tid = threadIdx.x, n = blockDim.x;
+  constexpr bool kTwo = MODE == kSwiglu || RES;
+  // SwiGLU's two inputs a value leave no registers for another row: with it requested ahead only one block
+  // fits an SM at 11008 columns (70 us for 4096 rows against 50 with a block a row)
+  constexpr bool kAhead = MODE != kSwiglu;
+  Raw8<T> first[VPT], second[kTwo ? VPT : 1];
+  Raw8<WT> wv[MODE == kNorm ? VPT : 1];
+  auto request = [&](long row) {
+    const T* x = (const T*)a.x + row * a.xs;
+    const T* r = RES ? (const T*)a.res + row * a.rs : x + a.D;
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = ((i0 + i) * n + tid) * 8;
-        if (c < a.D) {
-          xv[i].load(x + c);
-          if (MODE == kSwiglu) second[i].load(x + a.D + c);
-          if (MODE == kNorm && res) second[i].load(r + c);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = ((i0 + i) * n + tid) * 8;
-        if (c < a.D) {
-          xv[i].get(t[i]);
-          if (MODE == kSwiglu) {
-            float u[8];
-            second[i].get(u);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) t[i][j] = siluf_(t[i][j]) * u[j];
-          }
-          if (MODE == kNorm) {
-            Raw8<WT> wr;
-            wr.load(w + c);
-            if (res) {
-              float u[8];
-              second[i].get(u);
-#pragma unroll
-              for (int j = 0; j < 8; ++j) t[i][j] += u[j];
-              xv[i].set(t[i]);
-              if (out) xv[i].store(h + c);
-            }
-            float wv[8];
-            wr.get(wv);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              sum += t[i][j] * t[i][j];
-              t[i][j] = __fmul_rn(t[i][j], wv[j]);
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) t[i][j] = 0.f;
-        }
-      }
-    } else {
-      float second[MODE == kPlain ? 1 : VPT * 8], wv[MODE == kNorm ? VPT * 8 : 1];
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const int c = (i0 + i) * n + tid;
-        const bool in = c < a.D;
-        t[i / 8][i % 8] = in ? to_f(x[c]) : 0.f;
-        if (MODE == kSwiglu) second[i] = in ? to_f(x[a.D + c]) : 0.f;
-        if (MODE == kNorm) {
-          second[i] = in && res ? to_f(r[c]) : 0.f;
-          wv[i] = in ? to_f(w[c]) : 0.f;
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < S; ++i) {
-        const int c = (i0 + i) * n + tid;
-        float& v = t[i / 8][i % 8];
-        if (MODE == kSwiglu) v = siluf_(v) * second[i];
-        if (MODE == kNorm) {
-          if (res) {
-            v = round_to(v + second[i], h);
-            if (out && c < a.D) from_f(v, h + c);
-          }
-          sum += v * v;
-          v = __fmul_rn(v, wv[i]);
-        }
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (i * n + tid) * 8;
+      if (c < a.D) {
+        first[i].load(x + c);
+        if (kTwo) second[i].load(r + c);
       }
     }
   };
-  const int rounds = KEEP ? 1 : (a.D + W * S * n - 1) / (W * S * n);
-#pragma unroll 1
-  for (int k = 0; k < rounds; ++k) {
-    walk(k * S, true);
+  chain_ready();
+  chain_wait();
+  long row = blockIdx.x;
+  if (kAhead) request(row);
+  if (MODE == kNorm) {
 #pragma unroll
     for (int i = 0; i < VPT; ++i)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) most = amax_nan(most, t[i][j]);
-  }
-  uint32_t top = abs_bits(most);
-  block_stats(sum, top);
-  const Int8Grid grid = int8_grid(top);
-  if (tid == 0) {
-    const float rstd = MODE == kNorm ? __frsqrt_rn(__fdiv_rn(sum, (float)a.D) + a.eps) : 1.f;
-    const float amax = top < 0x00800000u ? 0.f : grid.amax;
-    a.scale[row] = __fdiv_rn(__fmul_rn(amax, rstd), 127.f);
+      if ((i * n + tid) * 8 < a.D) wv[i].load(w + (i * n + tid) * 8);
   }
 #pragma unroll 1
-  for (int k = 0; k < rounds; ++k) {
-    // the second walk reads x and r again, not h: they round to the same sum
-    if (!KEEP) walk(k * S, false);
-    if constexpr (VEC) {
+  for (int turn = 0; row < rows; row += gridDim.x, turn ^= 1) {
+    float t[VPT][8];
+    float sum = 0.f, most = 0.f;
+    if (!kAhead) request(row);
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        const int c = ((k * S + i) * n + tid) * 8;
-        uint32_t b[2];
-        int8_steps<8>(t[i], grid, b);
-        if (c < a.D) *reinterpret_cast<uint2*>(q + c) = make_uint2(b[0], b[1]);
-      }
-    } else {
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (i * n + tid) * 8;
+      if (c < a.D) {
+        first[i].get(t[i]);
+        float u[8];
+        if (kTwo) second[i].get(u);
+        if (MODE == kSwiglu) {
 #pragma unroll
-      for (int i = 0; i < VPT; ++i) {
-        uint32_t b[2];
-        int8_steps<8>(t[i], grid, b);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int c = (k * S + i * 8 + j) * n + tid;
-          if (c < a.D) q[c] = (int8_t)(b[j / 4] >> (8 * (j % 4)));
+          for (int j = 0; j < 8; ++j) t[i][j] = siluf_(t[i][j]) * u[j];
         }
+        if (MODE == kNorm) {
+          if (RES) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) t[i][j] += u[j];
+            first[i].set(t[i]);                              // the stream's own rounding
+            first[i].store((T*)a.h + row * a.hs + c);
+          }
+          float v[8];
+          wv[i].get(v);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            sum += t[i][j] * t[i][j];
+            t[i][j] = __fmul_rn(t[i][j], v[j]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t[i][j] = 0.f;
       }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = amax_nan(most, t[i][j]);
+    }
+    if (kAhead && row + gridDim.x < rows) request(row + gridDim.x);
+    uint32_t top = abs_bits(most);
+    block_stats<MODE == kNorm>(sum, top, turn);
+    const Int8Grid grid = int8_grid(top);
+    if (tid == 0) write_scale<MODE>(a, row, sum, top);
+    int8_t* q = a.q + row * a.qs;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int c = (i * n + tid) * 8;
+      const uint2 b = int8_steps(t[i], grid);
+      if (c < a.D) *reinterpret_cast<uint2*>(q + c) = b;
     }
   }
+}
+
+// Any alignment: a thread's values lie blockDim apart, so that a warp's accesses are contiguous.  KEEP: G
+// groups of eight of them stay in registers; otherwise the row is walked twice.
+template <int MODE, bool RES, typename T, typename WT, int G, bool KEEP>
+__global__ void __launch_bounds__(KEEP ? 512 : 1024) int8_rows_any_kernel(const RowArgs a) {
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x, n = blockDim.x;
+  const T* x = (const T*)a.x + row * a.xs + tid;
+  const T* r = (RES ? (const T*)a.res + row * a.rs : (const T*)a.x + row * a.xs + a.D) + tid;
+  const WT* w = (const WT*)a.w + tid;
+  constexpr bool kTwo = MODE == kSwiglu || RES;
+  float t[G][8];
+  float sum = 0.f, most = 0.f;
+  chain_ready();
+  chain_wait();
+  // eight accesses of this thread, n apart, from column c0 + tid on
+  auto walk = [&](float (&v)[8], int c0, bool out) {
+    float u[8], wv[8];
+    const int left = a.D - c0 - tid;                         // columns from this thread's first one on
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const bool in = j * n < left;
+      v[j] = in ? to_f(x[c0 + j * n]) : 0.f;
+      if (kTwo) u[j] = in ? to_f(r[c0 + j * n]) : 0.f;
+      if (MODE == kNorm) wv[j] = in ? to_f(w[c0 + j * n]) : 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (MODE == kSwiglu) v[j] = siluf_(v[j]) * u[j];
+      if (MODE == kNorm) {
+        if (RES) {
+          v[j] = round_to(v[j] + u[j], (const T*)nullptr);
+          if (out && j * n < left) from_f(v[j], (T*)a.h + row * a.hs + c0 + tid + j * n);
+        }
+        sum += v[j] * v[j];
+        v[j] = __fmul_rn(v[j], wv[j]);
+      }
+    }
+  };
+  const int groups = KEEP ? G : (a.D + 8 * n - 1) / (8 * n);
+#pragma unroll
+  for (int k = 0; k < groups; ++k) {
+    float (&v)[8] = t[KEEP ? k : 0];
+    walk(v, 8 * n * k, true);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) most = amax_nan(most, v[j]);
+  }
+  uint32_t top = abs_bits(most);
+  block_stats<MODE == kNorm>(sum, top, 0);
+  const Int8Grid grid = int8_grid(top);
+  if (tid == 0) write_scale<MODE>(a, row, sum, top);
+  int8_t* q = a.q + row * a.qs + tid;
+#pragma unroll
+  for (int k = 0; k < groups; ++k) {
+    float (&v)[8] = t[KEEP ? k : 0];
+    if (!KEEP) walk(v, 8 * n * k, false);                    // x and r again, not h: they round to the same sum
+    const uint2 b = int8_steps(v, grid);
+    const int left = a.D - 8 * n * k - tid;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (j * n < left) q[8 * n * k + j * n] = (int8_t)((j < 4 ? b.x : b.y) >> (8 * (j % 4)));
+  }
+}
+
+// Blocks of `kern` that the device holds at once.
+template <typename K>
+int resident(K kern, int threads) {
+  static int known[64][33] = {{0}};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64) return axh::sm_count();
+  int& k = known[dev][threads / 32];
+  if (k == 0) {
+    int n = 0;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
+    k = n * axh::sm_count();
+  }
+  return k;
 }
 
 // Threads and groups per thread: one group each for few rows (latency: all loads of the row are in flight
 // at once), four for many rows (a warp's share of the reduction and of the row's divisions is paid once per
 // 1024 values: 508 instructions a warp at two groups, of which 150 do not depend on them); rows up to 16384
 // wide stay in registers.
-template <int MODE, typename T, typename WT, bool VEC>
-int launch(const RowArgs& a, int rows, cudaStream_t stream) {
+template <int MODE, bool RES, typename T, typename WT>
+int launch_vec(const RowArgs& a, int rows, cudaStream_t stream) {
   const int groups = (a.D + 7) / 8;
-  int vpt = groups > 1024 ? 2 : 1;   // (the scalar path stops at two: its values are 8 x as many accesses)
-  if (rows > 2 * axh::sm_count() && groups > 64) vpt = VEC && groups >= 256 ? 4 : 2;
+  int vpt = groups > 1024 ? 2 : 1;
+  if (rows > 2 * axh::sm_count() && groups > 64) vpt = groups >= 256 ? 4 : 2;
   const int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
-  if (threads > (vpt == 4 ? 512 : 1024)) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 1, false, VEC>, dim3(rows), dim3(1024), 0, 1, stream, a);
-  if (vpt == 1) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 1, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
-  if (vpt == 2) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 2, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
-  if constexpr (VEC) return axh::launch_chained(int8_rows_kernel<MODE, T, WT, 4, true, VEC>, dim3(rows), dim3(threads), 0, 1, stream, a);
-  return -1;
+  auto go = [&](auto kern) {
+    const int most = MODE == kSwiglu ? rows : resident(kern, threads);
+    return axh::launch_chained(kern, dim3(rows < most ? rows : most), dim3(threads), 0, 1, stream, a, rows);
+  };
+  if (vpt == 1) return go(int8_rows_kernel<MODE, RES, T, WT, 1>);
+  if (vpt == 2) return go(int8_rows_kernel<MODE, RES, T, WT, 2>);
+  return go(int8_rows_kernel<MODE, RES, T, WT, 4>);
 }
 
-template <int MODE, typename T, typename WT>
-int launch_vec(const RowArgs& a, int rows, cudaStream_t stream) {
+template <int MODE, bool RES, typename T, typename WT>
+int launch(const RowArgs& a, int rows, cudaStream_t stream) {
   constexpr int kPer16 = 16 / (int)sizeof(T);
-  const bool vec = a.D % 8 == 0 && a.xs % kPer16 == 0 && a.rs % kPer16 == 0 && a.hs % kPer16 == 0 && a.qs % 8 == 0 &&
+  const bool vec = a.D % 8 == 0 && a.D <= 16384 && a.xs % kPer16 == 0 && a.rs % kPer16 == 0 && a.hs % kPer16 == 0 && a.qs % 8 == 0 &&
                    (((uintptr_t)a.x | (uintptr_t)a.res | (uintptr_t)a.h | (uintptr_t)a.w) & 15) == 0 && ((uintptr_t)a.q & 7) == 0;
-  return vec ? launch<MODE, T, WT, true>(a, rows, stream) : launch<MODE, T, WT, false>(a, rows, stream);
+  if (vec) return launch_vec<MODE, RES, T, WT>(a, rows, stream);
+  // one group of eight a thread up to 4096 columns, two up to 8192
+  const int threads = ((a.D + 7) / 8 + 31) / 32 * 32;
+  if (threads <= 512) return axh::launch_chained(int8_rows_any_kernel<MODE, RES, T, WT, 1, true>, dim3(rows), dim3(threads), 0, 1, stream, a);
+  if (threads <= 1024) {
+    const int half = ((a.D + 15) / 16 + 31) / 32 * 32;
+    return axh::launch_chained(int8_rows_any_kernel<MODE, RES, T, WT, 2, true>, dim3(rows), dim3(half), 0, 1, stream, a);
+  }
+  return axh::launch_chained(int8_rows_any_kernel<MODE, RES, T, WT, 1, false>, dim3(rows), dim3(1024), 0, 1, stream, a);
+}
+
+template <typename T, typename WT>
+int launch_norm(const RowArgs& a, int rows, cudaStream_t stream) {
+  return a.res != nullptr ? launch<kNorm, true, T, WT>(a, rows, stream) : launch<kNorm, false, T, WT>(a, rows, stream);
 }
 
 }  // namespace
@@ -229,11 +275,11 @@ AX_API int ax_int8_rows(int mode, int dt, int wdt, const void* x, long xs, const
   RowArgs a{x, res, w, h, q, scale, xs, rs, hs, qs, D, eps};
   using bf = __nv_bfloat16;
   if (mode == kNorm) {
-    if (dt == 1 && wdt == 1) return launch_vec<kNorm, bf, bf>(a, rows, stream);
-    if (dt == 1 && wdt == 0) return launch_vec<kNorm, bf, float>(a, rows, stream);
-    if (dt == 0 && wdt == 0) return launch_vec<kNorm, float, float>(a, rows, stream);
+    if (dt == 1 && wdt == 1) return launch_norm<bf, bf>(a, rows, stream);
+    if (dt == 1 && wdt == 0) return launch_norm<bf, float>(a, rows, stream);
+    if (dt == 0 && wdt == 0) return launch_norm<float, float>(a, rows, stream);
     return -2;
   }
-  if (mode == kSwiglu) return dt == 1 ? launch_vec<kSwiglu, bf, bf>(a, rows, stream) : launch_vec<kSwiglu, float, float>(a, rows, stream);
-  return dt == 1 ? launch_vec<kPlain, bf, bf>(a, rows, stream) : launch_vec<kPlain, float, float>(a, rows, stream);
+  if (mode == kSwiglu) return dt == 1 ? launch<kSwiglu, false, bf, bf>(a, rows, stream) : launch<kSwiglu, false, float, float>(a, rows, stream);
+  return dt == 1 ? launch<kPlain, false, bf, bf>(a, rows, stream) : launch<kPlain, false, float, float>(a, rows, stream);
 }

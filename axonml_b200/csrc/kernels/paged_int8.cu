@@ -86,16 +86,11 @@ __device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& 
   return false;
 }
 
-// rint(q a_old / a_new) of four bytes; the same border rule as int8_steps
-__device__ __forceinline__ uint32_t rescale4(uint32_t w, float old, float grown, float ratio) {
+// rint(q a_old / a_new) of four bytes
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, const Int8Grid& g) {
   uint32_t b[4];
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float q = (float)(int8_t)((w >> (8 * j)) & 255u), f = q * ratio;
-    float r = __fadd_rn(f, kRound);
-    if (fabsf(f - __fadd_rn(r, -kRound)) > kBorder) r = __fadd_rn(__fdiv_rn(__fmul_rn(q, old), grown), kRound);
-    b[j] = __float_as_uint(r);
-  }
+  for (int j = 0; j < 4; ++j) b[j] = int8_bits((float)(int8_t)((w >> (8 * j)) & 255u), g);
   return pack_low_bytes(b[0], b[1], b[2], b[3]);
 }
 
@@ -106,97 +101,112 @@ __device__ __forceinline__ uint32_t byte_mask(int w, int lo, int hi) {
   return below_b & ~below_a;
 }
 
-constexpr int kHalf = 64;     // threads of a block that work on K, and as many on V
-
-// Grid (pieces, Hkv): one block per page piece and head; half of its threads take K, half V.  The new
-// rows are read twice, the second time from L1: once for the magnitude, once to be rounded.
-// K: a thread rounds eight dims of a token.  V: four lanes take eight dims of sixteen slots, four slots each
-// (16-byte loads of four tokens), and exchange words so that each lane stores two dims' sixteen slots whole.
-template <typename T>
-__global__ void __launch_bounds__(2 * kHalf) kv_write_int8_kernel(const WriteArgs a) {
+// Grid (pieces, Hkv): a block takes a page piece of a head; kHalf of its threads take K, as many V.  A thread holds
+// four times eight dims, so that 16 tokens of 128 dims on 64 threads are read once and stay in registers between
+// the magnitude and the rounding; larger pieces are read a second time, from L1.
+// K: a thread rounds eight dims of a token.  V: four lanes take eight dims of sixteen slots, four slots each,
+// and exchange words so that each lane stores two dims' sixteen slots whole.
+template <typename T, int kHalf>
+__global__ void __launch_bounds__(2 * kHalf, 512 / kHalf) kv_write_int8_kernel(const WriteArgs a) {
   __shared__ uint32_t s_top[2 * kHalf / 32];
   chain_ready();
   chain_wait();
   Piece pc;
   if (!find_piece(a, (int)blockIdx.x, pc)) return;           // uniform over the block
-  const int h = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const bool is_v = threadIdx.x >= kHalf;
-  const int tid = threadIdx.x & (kHalf - 1);
-  const long ts = is_v ? a.v_ts : a.k_ts;
-  const T* x = (const T*)(is_v ? a.v : a.k) + (long)pc.src * ts + (long)h * (is_v ? a.v_hs : a.k_hs);
+  const int tid = threadIdx.x & (kHalf - 1), i4 = tid & 3;
+  const long ts = is_v ? a.v_ts : a.k_ts, hs = is_v ? a.v_hs : a.k_hs;
+  const T* rows = (const T*)(is_v ? a.v : a.k) + (long)pc.src * ts;
+  const int per_row = a.D / 8, end = pc.first + pc.count;
+
+  // K: threads side by side along a token's dims, 64 / per_row tokens at once, four of those a round.
+  // V: a unit is 16 slots x 8 dims on four lanes, 16 units a round.
+  const int g0 = pc.first / 16, g1 = (end + 15) / 16, units = (g1 - g0) * per_row;
+  const int across = kHalf / per_row, row0 = tid / per_row, tokens = 4 * across;
+  const int rounds = is_v ? (units + kHalf / 4 - 1) / (kHalf / 4) : (pc.count + tokens - 1) / tokens;
+  Raw8<T> raw[4];
+  int t0, step, col = (tid - row0 * per_row) * 8, slot0 = 0;  // this thread's tokens of the round: t0, t0 + step, ...
+  bool in = row0 < across;                                   // K: the thread has tokens; V: its unit exists
+  auto token = [&](int k) { return t0 + k * step; };
+  auto live = [&](int k) { return in && (unsigned)token(k) < (unsigned)pc.count; };
+  auto request = [&](const T* x, int round) {
+    if (is_v) {
+      const int u = round * (kHalf / 4) + tid / 4, g = u / per_row;
+      in = u < units;
+      col = (u - g * per_row) * 8;
+      slot0 = (g0 + g) * 16;                                 // the unit's first slot
+      t0 = slot0 + 4 * i4 - pc.first;
+      step = 1;
+    } else {
+      t0 = round * tokens + row0;
+      step = across;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (live(k)) raw[k].load(x + token(k) * ts + col);
+  };
+  const int h = blockIdx.y;
+  const T* x = rows + (long)h * hs;
   const long group = (long)pc.page * a.Hkv + h;
   float* amax_p = (is_v ? a.va : a.ka) + group;
   int8_t* dst = (is_v ? a.vc : a.kc) + group * a.P * a.D;
   const float before = pc.first > 0 ? *amax_p : 0.f;
-
   float most = 0.f;
-  const int per_row = a.D / 8, end = pc.first + pc.count;
-  // Both halves walk the rows as they lie; V's lanes come back to them in another order.
-#pragma unroll 4
-  for (int i = tid; i < pc.count * per_row; i += kHalf) {
-    const int t = i / per_row, c = (i - t * per_row) * 8;
-    Raw8<T> raw;
-    raw.load(x + t * ts + c);
-    float v[8];
-    raw.get(v);
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+    request(x, round);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) most = amax_nan(most, v[j]);
+    for (int k = 0; k < 4; ++k) {
+      if (live(k)) {
+        float v[8];
+        raw[k].get(v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) most = amax_nan(most, v[j]);
+      }
+    }
   }
   uint32_t top = __reduce_max_sync(0xffffffffu, abs_bits(most));
   if (lane == 0) s_top[warp] = top;
-  __syncthreads();                                           // also: every thread has read the old magnitude
+  __syncthreads();                                         // also: every thread has read the old magnitude
   const int w0 = is_v ? kHalf / 32 : 0;
 #pragma unroll
   for (int i = 0; i < kHalf / 32; ++i) top = max(top, s_top[w0 + i]);
-  const uint32_t old_bits = abs_bits(before) < 0x00800000u ? 0u : abs_bits(before);
+  const uint32_t old_bits = abs_bits(before) < kTinyBits ? 0u : abs_bits(before);
   top = max(top, old_bits);
-  if (top < 0x00800000u) top = 0;
+  if (top < kTinyBits) top = 0;
   const Int8Grid grid = int8_grid(top);
-  const float grown = __uint_as_float(top), old = __uint_as_float(old_bits);
-  const bool again = top > old_bits && pc.first > 0;
-  const float ratio = again && grid.live ? __fdiv_rn(old, grown) : 0.f;
-  if (tid == 0) *amax_p = grown;
+  const bool again = top > old_bits && pc.first > 0;       // the page's magnitude grows
+  const Int8Grid shrink = int8_grid(again ? top : 0u, __uint_as_float(old_bits));
+  if (tid == 0) *amax_p = __uint_as_float(top);
 
-  if (!is_v) {
-    if (again) {
-      uint2* rows = reinterpret_cast<uint2*>(dst);
-      for (int i = tid; i < pc.first * per_row; i += kHalf) {
-        const uint2 w = rows[i];
-        rows[i] = make_uint2(rescale4(w.x, old, grown, ratio), rescale4(w.y, old, grown, ratio));
-      }
+  if (again) {                                               // what the page held: whole tokens of K, whole 16-slot groups of V
+    uint4* held = reinterpret_cast<uint4*>(dst);
+    const int words = (is_v ? g0 * 16 : pc.first) * a.D / 16;
+#pragma unroll 1
+    for (int i = tid; i < words; i += kHalf) {
+      const uint4 w = held[i];
+      held[i] = make_uint4(rescale4(w.x, shrink), rescale4(w.y, shrink), rescale4(w.z, shrink), rescale4(w.w, shrink));
     }
-#pragma unroll 4
-    for (int i = tid; i < pc.count * per_row; i += kHalf) {
-      const int t = i / per_row, c = (i - t * per_row) * 8;
-      Raw8<T> raw;
-      raw.load(x + t * ts + c);
-      float v[8];
-      raw.get(v);
-      uint32_t b[2];
-      int8_steps<8>(v, grid, b);
-      *reinterpret_cast<uint2*>(dst + (long)(pc.first + t) * a.D + c) = make_uint2(b[0], b[1]);
-    }
-    return;
   }
-  const int g0 = again ? 0 : pc.first / 16, g1 = (end + 15) / 16;
-  const int i4 = tid & 3, units = (g1 - g0) * per_row;       // a unit: four lanes, sixteen slots, eight dims
-  for (int u0 = 0; u0 < units; u0 += kHalf / 4) {
-    const int u = u0 + tid / 4;
-    const bool in = u < units;
-    const int g = g0 + (in ? u / per_row : 0), c = in ? (u % per_row) * 8 : 0, s0 = g * 16;
-    uint32_t steps[4][2];                                    // [slot 4 i4 + .][dims 0-3 | 4-7]
+#pragma unroll 1
+  for (int round = 0; round < rounds; ++round) {
+    if (rounds > 1) request(x, round);
+    uint32_t steps[4][2];                                    // [token][dims 0-3 | 4-7]
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int slot = s0 + 4 * i4 + k;
       steps[k][0] = steps[k][1] = 0u;
-      if (in && slot >= pc.first && slot < end) {
-        Raw8<T> raw;
-        raw.load(x + (slot - pc.first) * ts + c);
+      if (live(k)) {
         float v[8];
-        raw.get(v);
-        int8_steps<8>(v, grid, steps[k]);
+        raw[k].get(v);
+        const uint2 b = int8_steps(v, grid);
+        steps[k][0] = b.x;
+        steps[k][1] = b.y;
+        if (!is_v) *reinterpret_cast<uint2*>(dst + (pc.first + token(k)) * a.D + col) = b;
       }
     }
+    if (!is_v) continue;
+    __syncwarp();
     // bytes [slot][dim] -> words word[dim] of this lane's four slots
     uint32_t word[8];
 #pragma unroll
@@ -208,33 +218,29 @@ __global__ void __launch_bounds__(2 * kHalf) kv_write_int8_kernel(const WriteArg
       word[4 * half + 2] = __byte_perm(hi01, hi23, 0x5410);
       word[4 * half + 3] = __byte_perm(hi01, hi23, 0x7632);
     }
-    // four lanes hold four slots each of dims c .. c + 7; lane i4 collects dims c + i4 and c + 4 + i4 in two
+    // four lanes hold four slots each of dims col .. col + 7; lane i4 collects dims col + i4 and col + 4 + i4 in two
     // exchanges (with the neighbour at distance 1, then 2)
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       uint32_t* m = word + 4 * half;
       const bool odd = i4 & 1, up = i4 & 2;
-      // distance 1: keep dims of this lane's parity
       const uint32_t s1 = __shfl_xor_sync(0xffffffffu, odd ? m[0] : m[1], 1), s2 = __shfl_xor_sync(0xffffffffu, odd ? m[2] : m[3], 1);
-      // a[d][lane parity]: dims {i4 & 1, 2 + (i4 & 1)}, slots of lanes (even, odd) of the pair
+      // dims {i4 & 1, 2 + (i4 & 1)}, slots of the pair's even and odd lane
       const uint32_t d0e = odd ? s1 : m[0], d0o = odd ? m[1] : s1;
       const uint32_t d2e = odd ? s2 : m[2], d2o = odd ? m[3] : s2;
-      // distance 2: lanes 0, 1 keep dims 0, 1; lanes 2, 3 keep dims 2, 3
+      // lanes 0, 1 keep dims 0, 1; lanes 2, 3 keep dims 2, 3
       const uint32_t r0 = __shfl_xor_sync(0xffffffffu, up ? d0e : d2e, 2), r1 = __shfl_xor_sync(0xffffffffu, up ? d0o : d2o, 2);
-      uint32_t out[4];
-      out[0] = up ? r0 : d0e;
-      out[1] = up ? r1 : d0o;
-      out[2] = up ? d2e : r0;
-      out[3] = up ? d2o : r1;
+      uint32_t out[4] = {up ? r0 : d0e, up ? r1 : d0o, up ? d2e : r0, up ? d2o : r1};
       if (in) {
-        uint4* p = reinterpret_cast<uint4*>(dst + (long)g * 16 * a.D + (c + 4 * half + i4) * 16);
+        const int s0 = slot0;
+        uint4* p = reinterpret_cast<uint4*>(dst + (long)s0 * a.D + (col + 4 * half + i4) * 16);
         if (s0 < pc.first || s0 + 16 > end) {                // slots that are neither old nor new keep their byte
           const uint4 o = *p;
           const uint32_t was[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const uint32_t fresh = byte_mask(k, pc.first - s0, end - s0), held = again ? byte_mask(k, 0, pc.first - s0) : 0u;
-            const uint32_t scaled = held ? rescale4(was[k], old, grown, ratio) : 0u;
+            const uint32_t scaled = held ? rescale4(was[k], shrink) : 0u;
             out[k] = (out[k] & fresh) | (scaled & held) | (was[k] & ~(fresh | held));
           }
         }
@@ -810,16 +816,20 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
                             float* ka, float* va, const int* table, const int* starts, const int* cu, int T, int B, int Hkv, int D, int P,
                             int max_pages, int num_pages, int* status, cudaStream_t stream) {
   if (T <= 0 || B <= 0 || Hkv <= 0) return 0;
-  if (D % 8 || P % 16 || P <= 0 || Hkv > 65535 || (cu == nullptr && T % B)) return -1;
+  if (D % 16 || D > 512 || P % 16 || P <= 0 || (long)P * D > (1L << 30) || Hkv > 65535 || (cu == nullptr && T % B)) return -1;
   const int vec = dt == 1 ? 8 : 4;
   if ((k_ts % vec) || (k_hs % vec) || (v_ts % vec) || (v_hs % vec) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)) return -2;
-  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, status};
   // a row of n tokens touches at most (n - 1) / P + 2 pages; a single token one
   const long rows = B < T ? B : T;
   const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
+  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, status};
   const dim3 grid((unsigned)pieces, Hkv);
-  if (dt == 1) return axh::launch_chained(kv_write_int8_kernel<__nv_bfloat16>, grid, dim3(2 * kHalf), 0, 1, stream, a);
-  return axh::launch_chained(kv_write_int8_kernel<float>, grid, dim3(2 * kHalf), 0, 1, stream, a);
+  // Larger blocks shorten the latency of a big page where few blocks leave room (200 tokens, pages of 64 x 128: 6.2 us
+  // against 8.4); full devices prefer the small ones (8192 tokens, pages of 16 x 128: 19.5 against 32.1).
+  const bool big = (long)P * D >= 4096 && pieces * Hkv < 8L * axh::sm_count();
+  auto go = [&](auto kern, int half) { return axh::launch_chained(kern, grid, dim3(2 * half), 0, 1, stream, a); };
+  if (dt == 1) return big ? go(kv_write_int8_kernel<__nv_bfloat16, 128>, 128) : go(kv_write_int8_kernel<__nv_bfloat16, 64>, 64);
+  return big ? go(kv_write_int8_kernel<float, 128>, 128) : go(kv_write_int8_kernel<float, 64>, 64);
 }
 
 // How the attention kernel is launched for a cache of this capacity.

@@ -3,7 +3,8 @@ int8 matrix (``csrc/kernels/int8_rows.cu``, ``int8_gemm.cu``).
 
 A value is ``q * scale`` with ``q`` in [-127, 127] and one fp32 scale per row (a token of the
 activations, an output channel of a weight).  The producers round as the real numbers would:
-``q = rint(127 y / max|y|)``, ties to even.  For inference; nothing here has a gradient.  CPU tensors
+``q = rint(127 y / max|y|)``, ties to even; a row below ``TINY`` everywhere counts as zero, one with
+a value that is not finite gets a scale that is not.  For inference; nothing here has a gradient.  CPU tensors
 take the same maths in torch."""
 from __future__ import annotations
 
@@ -34,13 +35,18 @@ def _no_gradient() -> None:
         raise RuntimeError("the int8 operators have no gradient: call them under torch.no_grad()")
 
 
+TINY = 2.0 ** -120      # a group whose largest magnitude is below this counts as zero
+
+
 def _steps(t: torch.Tensor, amax: torch.Tensor) -> torch.Tensor:
     one = torch.where(amax > 0, amax, torch.ones_like(amax))
-    return torch.where(amax > 0, (t * 127.0 / one).round(), torch.zeros_like(t)).nan_to_num_(0.0).to(torch.int8)
+    q = (t.double() * 127.0 / one.double()).round()
+    return torch.where(amax > 0, q, torch.zeros_like(q)).nan_to_num_(0.0).to(torch.int8)
 
 
 def _ref_rows(t: torch.Tensor, norm=None):
     amax = t.abs().amax(-1, keepdim=True) if t.shape[-1] else t.new_zeros(t.shape[:-1] + (1,))
+    amax = torch.where(amax < TINY, torch.zeros_like(amax), amax)
     scale = (amax if norm is None else amax * norm) / 127.0
     return _steps(t, amax), scale.squeeze(-1).float()
 
@@ -71,7 +77,7 @@ def _launch_rows(mode: int, x: torch.Tensor, D: int, res=None, weight=None, eps:
         wp, wk = weight.data_ptr(), _kind(weight.dtype, "weight")
     if res is not None:
         r2 = res if flat and res.stride(1) == 1 else _rows2d(res)
-        h = torch.empty((rows, D), dtype=dtype, device=dev)
+        h = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((rows, D), dtype=dtype, device=dev)
         rp, rs, hp = r2.data_ptr(), r2.stride(0), h.data_ptr()
     if rows:
         N.launch("ax_int8_rows", dev.index, mode, kind, wk, x2.data_ptr(), x2.stride(0), rp, rs, wp, eps, hp, D, q.data_ptr(), q.stride(0),

@@ -9,6 +9,7 @@ import math
 import torch
 
 from .. import _native as N
+from .int8 import TINY
 
 
 def kv_write(k, v, k_cache, v_cache, block_table, seq_ids, positions, page_size: int) -> None:
@@ -122,6 +123,8 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
         return
     if k.dtype not in (torch.bfloat16, torch.float32):
         raise TypeError(f"k and v must be bf16 or fp32 on a GPU, not {k.dtype}")
+    if D > 512 or Hkv > 65535 or P * D > 1 << 30:
+        raise ValueError(f"head_dim {D}, {Hkv} KV heads or page_size {P} are more than the kernel takes (512, 65535, 2^30 / head_dim)")
     if T == 0 or B == 0:
         return
     vec = 16 // k.element_size()
@@ -157,11 +160,12 @@ def _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, star
                 new = x[src:src + cnt].transpose(0, 1).float()
                 old = amax[page].clone() if lo else torch.zeros_like(amax[page])
                 grown = torch.maximum(old, new.abs().amax((1, 2)))
-                one = torch.where(grown > 0, grown, torch.ones_like(grown))[:, None, None]
+                grown = torch.where(grown < TINY, torch.zeros_like(grown), grown)
+                one = torch.where(grown > 0, grown, torch.ones_like(grown)).double()[:, None, None]
                 if lo:
-                    kept = (rows[:, :lo].float() * old[:, None, None] / one).round().nan_to_num_(0.0).to(torch.int8)
+                    kept = (rows[:, :lo].double() * old[:, None, None] / one).round().nan_to_num_(0.0).to(torch.int8)
                     rows[:, :lo] = torch.where((grown > old)[:, None, None], kept, rows[:, :lo])
-                rows[:, lo:lo + cnt] = (new * 127.0 / one).round().nan_to_num_(0.0).to(torch.int8)
+                rows[:, lo:lo + cnt] = (new.double() * 127.0 / one).round().nan_to_num_(0.0).to(torch.int8)
                 amax[page] = grown
                 if is_v:
                     cache[page] = rows.view(-1, P // 16, 16, D).transpose(-1, -2)
