@@ -210,9 +210,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) int8_rows_any_kernel(const 
   }
 }
 
-// Blocks of `kern` that the device holds at once.
-template <typename K>
-int resident(K kern, int threads) {
+// Blocks of Kern that the device holds at once.
+template <auto Kern>
+int resident(int threads) {
   static int known[64][33] = {{0}};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -220,10 +220,15 @@ int resident(K kern, int threads) {
   int& k = known[dev][threads / 32];
   if (k == 0) {
     int n = 0;
-    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, threads, 0) != cudaSuccess || n < 1) n = 1;
+    if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, Kern, threads, 0) != cudaSuccess || n < 1) n = 1;
     k = n * axh::sm_count();
   }
   return k;
+}
+template <auto Kern>
+int launch_rows(const RowArgs& a, int rows, int threads, bool ahead, cudaStream_t stream) {
+  const int most = ahead ? resident<Kern>(threads) : rows;   // a kernel that does not request ahead takes a block a row
+  return axh::launch_chained(Kern, dim3(rows < most ? rows : most), dim3(threads), 0, 1, stream, a, rows);
 }
 
 // Threads and groups per thread: one group each for few rows (latency: all loads of the row are in flight
@@ -236,13 +241,9 @@ int launch_vec(const RowArgs& a, int rows, cudaStream_t stream) {
   int vpt = groups > 1024 ? 2 : 1;
   if (rows > 2 * axh::sm_count() && groups > 64) vpt = groups >= 256 ? 4 : 2;
   const int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
-  auto go = [&](auto kern) {
-    const int most = MODE == kSwiglu ? rows : resident(kern, threads);
-    return axh::launch_chained(kern, dim3(rows < most ? rows : most), dim3(threads), 0, 1, stream, a, rows);
-  };
-  if (vpt == 1) return go(int8_rows_kernel<MODE, RES, T, WT, 1>);
-  if (vpt == 2) return go(int8_rows_kernel<MODE, RES, T, WT, 2>);
-  return go(int8_rows_kernel<MODE, RES, T, WT, 4>);
+  if (vpt == 1) return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 1>>(a, rows, threads, MODE != kSwiglu, stream);
+  if (vpt == 2) return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 2>>(a, rows, threads, MODE != kSwiglu, stream);
+  return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 4>>(a, rows, threads, MODE != kSwiglu, stream);
 }
 
 template <int MODE, bool RES, typename T, typename WT>

@@ -44,7 +44,7 @@ __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start,
     src = b * len;
   }
   if (len <= 0) return 0;
-  if (start < 0 || src < 0 || src + len > a.T || (long)start + len > (long)a.max_pages * a.P) {
+  if (start < 0 || src < 0 || (long)src + len > a.T || (long)start + len > min((long)a.max_pages * a.P, 0x7fffffffL)) {
     set_status(a.status, kBadArgument, 1200);
     return 0;
   }
@@ -289,9 +289,9 @@ __device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) {
   const long cap = (long)a.max_pages * a.P;
   if (n < 0 || n > cap) {
     set_status(a.status, kBadArgument, 1210);
-    n = n < 0 ? 0 : (int)cap;
+    n = n < 0 ? 0 : (int)cap;                                    // (below n, so it fits)
   }
-  return (n + kTile - 1) / kTile;
+  return n / kTile + (n % kTile != 0);
 }
 __device__ __forceinline__ int chunk_of(const AttnArgs& a, int total) {
   const int even = (total + a.workers - 1) / a.workers;
@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
 #pragma unroll 1
   for (int t = 0; t < n;) {
     // ---- a head: all or part of its tokens
-    ctx = min(a.ctx[b], a.max_pages * a.P);
+    ctx = (int)min((long)a.ctx[b], (long)a.max_pages * a.P);
     const int h0 = (vh / a.nblk) * a.G, first = (vh % a.nblk) * HG;
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {

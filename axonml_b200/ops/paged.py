@@ -104,8 +104,8 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
     ``block_table`` ``[B, max_pages]``) brings tokens ``cu_seqlens[b] .. cu_seqlens[b + 1]`` (without
     ``cu_seqlens``: ``T / B`` each) at positions ``starts[b], starts[b] + 1, ...``; rows of ``k`` / ``v`` behind
     ``cu_seqlens[B]`` are ignored.  A page's magnitude grows to the largest value it holds, and what it held
-    before is rounded to the new grid; a page written from its first slot starts anew.  Two sequences
-    of one call must not write to the same page.  On a GPU a sequence that does not fit its table or a
+    before is rounded to the new grid; a page written from its first slot starts anew.  ``cu_seqlens`` must not
+    decrease, and two sequences of one call must not write to the same page.  On a GPU a sequence that does not fit its table or a
     page number outside the cache is skipped and reported by ``_native.check_status()``."""
     pages, Hkv, P, D = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
     if k.dim() != 3 or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:

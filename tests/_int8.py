@@ -72,7 +72,7 @@ def attention(q, k_rows, v_rows_, ka, va, table, ctx, scale):
         # small elements kept to 2^-24 of the row's largest; half again for the maximum that all scores are compared with
         mag = torch.einsum("hgd,hnd->hgn", qq.abs(), k.abs()).amax(-1)
         tiny = qq.abs().amax(-1) * k.abs().sum(-1).amax(-1, keepdim=True)
-        ds = 2 * scale * ((16 + D / 16) * 2.0 ** -22 * mag + 4 * 2.0 ** -24 * mag + 2.0 ** -24 * tiny)
+        ds = 2 * abs(scale) * ((16 + D / 16) * 2.0 ** -22 * mag + 4 * 2.0 ** -24 * mag + 2.0 ** -24 * tiny)
         # a weight: fp16's half step 2^-11, exp2's 2^-21, fp32 sums of them.  Below 2^-14 fp16 keeps 2^-25; the weight is stored times
         # its page's V magnitude over the largest page's, at least 1/8, and the largest weight is at least one: 8 * 2^-25 of that
         ew = 2 * ds + 2.0 ** -11 + 2.0 ** -20

@@ -116,7 +116,7 @@ def test_attention_extreme_scores_and_scales(kernel_status):
     va[table[0, 4]] = 0.0
     va[table[0, 5]] *= 1000
     cl = torch.tensor([n], dtype=torch.int32).cuda()
-    for scale in (None, 0.5, 1e-4):
+    for scale in (None, 0.5, 1e-4, -0.3, 0.0):
         got = paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl, scale)
         want, off = R.attention(q, kc, R.v_rows(vc), ka, va, table.tolist(), [n], R.default_scale(D) if scale is None else scale)
         assert ((got.double() - want).abs() <= off + torch.finfo(torch.bfloat16).eps / 2 * (want.abs() + off)).all()
@@ -190,6 +190,84 @@ def test_write_then_attend_in_a_graph_and_on_another_stream(kernel_status):
         assert torch.equal(out, want)
     for a, b in zip(caches, eager):
         assert torch.equal(a, b)
+
+
+def test_captured_branches_memsets_and_copies(kernel_status):
+    """The operators as first and as joining nodes of a captured fork, behind a memset and a copy, replayed several times."""
+    from axonml_b200.ops import int8 as I
+    x = torch.randn(300, 512, device="cuda").bfloat16()
+    w = torch.ones(512, device="cuda").bfloat16()
+    W = I.Int8Weight.from_dense(torch.randn(384, 512, device="cuda"))
+    src, buf = torch.zeros_like(x), torch.zeros_like(x)
+
+    def steps(side):
+        here = torch.cuda.current_stream()
+        buf.zero_()
+        a = I.rms_norm_int8(buf, w, residual=x)               # behind a memset
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            b = I.int8_linear(*I.quantize_int8(x), W.q, W.scale)          # first of a branch
+        buf.copy_(src)
+        c = I.int8_linear(a[0], a[1], W.q, W.scale)           # behind a copy, beside the branch
+        here.wait_stream(side)
+        d = I.rms_norm_int8(c, torch.ones(384, device="cuda").bfloat16(), residual=b)     # joins both
+        return [*a, b, c, *d]
+    side = torch.cuda.Stream()
+    steps(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = steps(side)
+    for _ in range(3):
+        x.copy_(torch.randn(300, 512))
+        src.copy_(torch.randn(300, 512))
+        for _ in range(4):
+            g.replay()
+        torch.cuda.synchronize()
+        want = steps(side)
+        torch.cuda.synchronize()
+        for p, q in zip(out, want):
+            assert torch.equal(p, q)
+
+
+def test_two_calls_at_once(kernel_status):
+    """The same operators on two streams at the same time, each with its own inputs."""
+    Hkv, G, D, P = 4, 4, 128, 16
+    ctx = [1500, 3, 900]
+    table, pages = _table([(n + P - 1) // P for n in ctx])
+    cl, tab = torch.tensor(ctx, dtype=torch.int32).cuda(), table.cuda()
+    sets = [R.make_cache(pages, Hkv, P, D, "cuda", seed=s) + [torch.randn(3, Hkv * G, D, device="cuda").bfloat16()] for s in (1, 2)]
+    alone = [paged.decode_attention_int8(c[4], *c[:4], tab, cl) for c in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for i, (c, s) in enumerate(zip(sets, streams)):
+            with torch.cuda.stream(s):
+                got[i].append(paged.decode_attention_int8(c[4], *c[:4], tab, cl))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(x, alone[i]) for x in got[i])
+
+
+def test_capture_before_the_first_call_is_refused():
+    """The status word is made outside captures."""
+    from axonml_b200 import _native as N
+    saved, words = dict(N._STATUS_PTR), dict(N._STATUS)
+    W = torch.zeros(32, 32, dtype=torch.int8, device="cuda")
+    s = torch.ones(32, device="cuda")
+    from axonml_b200.ops import int8 as I
+    g = torch.cuda.CUDAGraph()
+    try:
+        N._STATUS_PTR.clear()
+        N._STATUS.clear()
+        with pytest.raises(N.NativeError):
+            with torch.cuda.graph(g):
+                I.int8_linear(W, s, W, s)
+    finally:
+        N._STATUS_PTR.update(saved)
+        N._STATUS.update(words)
+    torch.cuda.synchronize()
 
 
 def _gpu_model(**kw):
