@@ -11,8 +11,8 @@
 // next row is requested before that reduction, so that its loads travel while this row is rounded.  Rows too
 // wide for registers are read twice, the second time from L2.  The kernels are bound by the bytes of x, r, h
 // and q, in so far as a row's 15 to 24 instructions a value leave room: norm of 8192 x 4096 bf16 with a
-// residual 37.9 us (6.2 TB/s), SwiGLU of 4096 x 11008 51.5 us (4.4 TB/s: two special-function results a value, and
-// 704 threads an SM), 1021 x 5125 fp32 rows off the 16-byte grid 11 us.
+// residual 37.9 us (6.2 TB/s), SwiGLU of 4096 x 11008 45.2 us (5.0 TB/s: two special-function results and some 20
+// instructions a value), 1021 x 5125 fp32 rows off the 16-byte grid 11 us.
 #include "int8_common.cuh"
 
 namespace {
@@ -147,6 +147,46 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSw
   }
 }
 
+// SwiGLU of many wide rows: the gated values wait in shared memory (D floats), not in registers, so that enough
+// warps are there to load other rows meanwhile.
+template <typename T>
+__global__ void __launch_bounds__(512) swiglu_int8_rows_kernel(const RowArgs a) {
+  extern __shared__ float4 held[];                           // [2][groups]: values 0-3 and 4-7 of every group of eight
+  const long row = blockIdx.x;
+  const int tid = threadIdx.x, groups = a.D / 8;
+  const T* x = (const T*)a.x + row * a.xs;
+  chain_ready();
+  chain_wait();
+  float most = 0.f, none = 0.f;
+#pragma unroll 3
+  for (int i = tid; i < groups; i += 512) {
+    Raw8<T> g, u;
+    g.load(x + 8 * i);
+    u.load(x + a.D + 8 * i);
+    float v[8], w[8];
+    g.get(v);
+    u.get(w);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = siluf_(v[j]) * w[j];
+      most = amax_nan(most, v[j]);
+    }
+    held[i] = make_float4(v[0], v[1], v[2], v[3]);
+    held[groups + i] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+  uint32_t top = abs_bits(most);
+  block_stats<false>(none, top, 0);
+  const Int8Grid grid = int8_grid(top);
+  if (tid == 0) write_scale<kSwiglu>(a, row, 0.f, top);
+  int8_t* q = a.q + row * a.qs;
+#pragma unroll 3
+  for (int i = tid; i < groups; i += 512) {
+    const float4 p = held[i], r = held[groups + i];
+    const float v[8] = {p.x, p.y, p.z, p.w, r.x, r.y, r.z, r.w};
+    *reinterpret_cast<uint2*>(q + 8 * i) = int8_steps(v, grid);
+  }
+}
+
 // Any alignment: a thread's values lie blockDim apart, so that a warp's accesses are contiguous.  KEEP: G
 // groups of eight of them stay in registers; otherwise the row is walked twice.
 template <int MODE, bool RES, typename T, typename WT, int G, bool KEEP>
@@ -241,6 +281,22 @@ int launch_vec(const RowArgs& a, int rows, cudaStream_t stream) {
   int vpt = groups > 1024 ? 2 : 1;
   if (rows > 2 * axh::sm_count() && groups > 64) vpt = groups >= 256 ? 4 : 2;
   const int threads = ((groups + vpt - 1) / vpt + 31) / 32 * 32;
+  if constexpr (MODE == kSwiglu) {
+    // Values in shared memory where registers would leave one or two blocks an SM.  Registers / shared memory, us:
+    // 4096 rows of bf16, 8192 wide 31.3 / 36.9, 9728 40.4 / 41.9, 11008 51.5 / 45.2, 14336 60.2 / 57.6; fp32, 4096 wide
+    // 35.8 / 25.3, 8192 67.1 / 45.8.
+    if (vpt == 4 && a.D >= (sizeof(T) == 2 ? 10240 : 4096)) {
+      static bool configured[64] = {false};
+      int dev = 0;
+      cudaGetDevice(&dev);
+      if (dev < 0 || dev >= 64 || !configured[dev]) {
+        cudaError_t e = cudaFuncSetAttribute(swiglu_int8_rows_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, 16384 * 4);
+        if (e != cudaSuccess) return (int)e;
+        if (dev >= 0 && dev < 64) configured[dev] = true;
+      }
+      return axh::launch_chained(swiglu_int8_rows_kernel<T>, dim3(rows), dim3(512), a.D * 4, 1, stream, a);
+    }
+  }
   if (vpt == 1) return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 1>>(a, rows, threads, MODE != kSwiglu, stream);
   if (vpt == 2) return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 2>>(a, rows, threads, MODE != kSwiglu, stream);
   return launch_rows<int8_rows_kernel<MODE, RES, T, WT, 4>>(a, rows, threads, MODE != kSwiglu, stream);

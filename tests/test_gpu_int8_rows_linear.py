@@ -36,7 +36,7 @@ def test_rms_norm_rows(rows, D, dt, wdt, res, kernel_status):
     _check_rows(got[0], got[1], hd * w.double(), torch.rsqrt(hd.pow(2).mean(-1, keepdim=True) + 1e-5), off, (81 / 2 + 6) * U)
 
 
-@pytest.mark.parametrize("rows,F", [(1, 16), (2, 5), (64, 14336), (300, 11008), (3, 1021), (1, 40000), (900, 256)])
+@pytest.mark.parametrize("rows,F", [(1, 16), (2, 5), (64, 14336), (300, 11008), (3, 1021), (1, 40000), (900, 256), (300, 4096), (297, 16384)])
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_swiglu_and_plain_rows(rows, F, dt, kernel_status):
     gu = torch.randn(rows, 2 * F, device="cuda").to(dt)
