@@ -19,10 +19,7 @@ MAX_K = 131071          # 2^14 K < 2^31: the int32 sum cannot overflow
 
 def _aligned_rows(rows: int, cols: int, device) -> torch.Tensor:
     """int8 ``[rows, cols]`` whose rows start on 16-byte boundaries (the product's loads need that)."""
-    pad = -cols % 16
-    if not pad:
-        return torch.empty((rows, cols), dtype=torch.int8, device=device)
-    return torch.empty((rows, cols + pad), dtype=torch.int8, device=device)[:, :cols]
+    return torch.empty_strided((rows, cols), (cols + -cols % 16, 1), dtype=torch.int8, device=device)
 
 
 def _rows2d(t: torch.Tensor) -> torch.Tensor:
@@ -51,6 +48,7 @@ def _ref_rows(t: torch.Tensor, norm=None):
     return _steps(t, amax), scale.squeeze(-1).float()
 
 
+_I8, _F32 = torch.int8, torch.float32
 _KINDS = {torch.bfloat16: 1, torch.float32: 0}
 
 
@@ -63,24 +61,33 @@ def _kind(dtype: torch.dtype, what: str) -> int:
 
 def _launch_rows(mode: int, x: torch.Tensor, D: int, res=None, weight=None, eps: float = 0.0):
     flat = x.dim() == 2
-    x2 = x if flat and x.stride(1) == 1 else _rows2d(x)
-    rows, dev, dtype = x2.shape[0], x.device, x.dtype
+    strides = x.stride() if flat else (0, 0)
+    if strides[1] == 1:
+        x2 = x
+    else:
+        x2 = _rows2d(x)
+        strides = x2.stride()
+    rows, dtype, index = x2.shape[0], x.dtype, x.get_device()
     wk = kind = _kind(dtype, "x")
-    q = _aligned_rows(rows, D, dev)
-    scale = torch.empty(rows, dtype=torch.float32, device=dev)
+    if D % 16 == 0 and mode != 2 and strides[0] == D:
+        q = torch.empty_like(x2, dtype=_I8)
+    else:
+        q = _aligned_rows(rows, D, x.device)
+    scale = x2.new_empty(rows, dtype=_F32)
     h, rp, rs, hp, wp = None, 0, 0, 0, 0
     if weight is not None:
-        if weight.dtype != torch.float32 and weight.dtype != dtype:
-            weight = weight.float()
+        wt = weight.dtype
+        if wt is not _F32 and wt is not dtype:
+            weight, wt = weight.float(), _F32
         if not weight.is_contiguous():
             weight = weight.contiguous()
-        wp, wk = weight.data_ptr(), _kind(weight.dtype, "weight")
+        wp, wk = weight.data_ptr(), _KINDS[wt]
     if res is not None:
         r2 = res if flat and res.stride(1) == 1 else _rows2d(res)
-        h = torch.empty_like(x2) if x2.is_contiguous() else torch.empty((rows, D), dtype=dtype, device=dev)
+        h = torch.empty_like(x2) if strides[0] == D else torch.empty((rows, D), dtype=dtype, device=x.device)
         rp, rs, hp = r2.data_ptr(), r2.stride(0), h.data_ptr()
     if rows:
-        N.launch("ax_int8_rows", dev.index, mode, kind, wk, x2.data_ptr(), x2.stride(0), rp, rs, wp, eps, hp, D, q.data_ptr(), q.stride(0),
+        N.launch("ax_int8_rows", index, mode, kind, wk, x2.data_ptr(), strides[0], rp, rs, wp, eps, hp, D, q.data_ptr(), q.stride(0),
                  scale.data_ptr(), rows, D)
     if not flat:
         lead = x.shape[:-1]
@@ -111,15 +118,15 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
     """RMSNorm over the last dim, to int8 rows: ``(q, scale)``.  With ``residual`` the norm is of
     ``h = x + residual`` (rounded to ``x``'s type) and the result is ``(q, scale, h)``."""
     _check_rows(x)
-    D, dev = x.shape[-1], x.device
+    D, dev = x.shape[-1], x.get_device()                   # (-1: not on a GPU)
     if weight.dim() != 1 or weight.shape[0] != D:
         raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {D}")
-    if weight.device != dev:
-        raise ValueError(f"weight is on {weight.device}, x on {dev}")
+    if weight.get_device() != dev:
+        raise ValueError(f"weight is on {weight.device}, x on {x.device}")
     if weight.requires_grad:
         _no_gradient()
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype or residual.device != dev:
+        if residual.shape != x.shape or residual.dtype is not x.dtype or residual.get_device() != dev:
             raise ValueError("residual must have x's shape, type and device")
         if residual.requires_grad:
             _no_gradient()
@@ -156,45 +163,49 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
     ``weight`` int8 ``[N, K]`` with ``weight_scale`` ``[N]``.  The integer sum is exact; the result is
     rounded once, to ``out_dtype`` (bf16 or fp32).  K is at most 131071.  Operands whose rows do not start
     on 16-byte boundaries are copied first; ``quantize_int8`` and the fused producers lay them out so."""
-    if q.dtype != torch.int8 or weight.dtype != torch.int8:
+    if q.dtype is not _I8 or weight.dtype is not _I8:
         raise TypeError("q and weight must be int8")
-    lead = q.shape[:-1]
+    flat = q.dim() == 2
     if weight.dim() != 2 or q.dim() < 1 or q.shape[-1] != weight.shape[1]:
         raise ValueError(f"q {tuple(q.shape)} does not fit a weight {tuple(weight.shape)}")
     Nn, K = weight.shape
     if not 0 < K <= MAX_K:
         raise ValueError(f"K must be in 1..{MAX_K}, not {K}")
-    if scale.shape != lead or weight_scale.dim() != 1 or weight_scale.shape[0] != Nn:
+    q2 = q if flat else q.reshape(-1, K)
+    M = q2.shape[0]
+    fits = scale.dim() == 1 and scale.shape[0] == M if flat else scale.shape == q.shape[:-1]
+    if not fits or weight_scale.dim() != 1 or weight_scale.shape[0] != Nn:
         raise ValueError(f"scales {tuple(scale.shape)}, {tuple(weight_scale.shape)} do not fit {tuple(q.shape)}, {tuple(weight.shape)}")
-    if scale.dtype != torch.float32 or weight_scale.dtype != torch.float32:
+    if scale.dtype is not _F32 or weight_scale.dtype is not _F32:
         raise TypeError("scales must be fp32")
-    if out_dtype not in _KINDS:
+    kind = _KINDS.get(out_dtype)
+    if kind is None:
         raise TypeError(f"out_dtype must be bf16 or fp32, not {out_dtype}")
-    dev = q.device
+    index = q.get_device()                                 # (-1: not on a GPU)
     if bias is not None:
-        if bias.dim() != 1 or bias.shape[0] != Nn or bias.device != dev:
-            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not fit {Nn} channels on {dev}")
+        if bias.dim() != 1 or bias.shape[0] != Nn or bias.get_device() != index:
+            raise ValueError(f"bias {tuple(bias.shape)} on {bias.device} does not fit {Nn} channels on {q.device}")
         if bias.requires_grad:
             _no_gradient()
-    if scale.device != dev or weight.device != dev or weight_scale.device != dev:
-        raise ValueError(f"q is on {dev}, its scale on {scale.device}, the weight on {weight.device}, its scale on {weight_scale.device}")
+    if scale.get_device() != index or weight.get_device() != index or weight_scale.get_device() != index:
+        raise ValueError(f"q is on {q.device}, its scale on {scale.device}, the weight on {weight.device}, its scale on {weight_scale.device}")
     if scale.requires_grad or weight_scale.requires_grad:
         _no_gradient()
-    q2 = q if q.dim() == 2 else q.reshape(-1, K)
-    if not q.is_cuda:
+    if index < 0:
         y = (q2.double() @ weight.double().t()).float() * scale.reshape(-1, 1) * weight_scale
         y = y if bias is None else y + bias.float()
-        return y.to(out_dtype).view(*lead, Nn)
-    M = q2.shape[0]
-    out = torch.empty((M, Nn), dtype=out_dtype, device=dev)
+        return y.to(out_dtype).view(*q.shape[:-1], Nn)
+    out = torch.empty_strided((M, Nn), (Nn, 1), dtype=out_dtype, device=q.device)
     if M and Nn:
-        qs, ws = q2.stride(0), weight.stride(0)
-        if q2.stride(1) != 1 or qs % 16 or q2.data_ptr() % 16:
-            q2 = _aligned_rows(M, K, dev).copy_(q2)
-            qs = q2.stride(0)
-        if weight.stride(1) != 1 or ws % 16 or weight.data_ptr() % 16:
-            weight = _aligned_rows(Nn, K, dev).copy_(weight)
-            ws = weight.stride(0)
+        qs, q1 = q2.stride()
+        ws, w1 = weight.stride()
+        qp, wp = q2.data_ptr(), weight.data_ptr()
+        if q1 != 1 or qs % 16 or qp % 16:
+            q2 = _aligned_rows(M, K, q.device).copy_(q2)
+            qs, qp = q2.stride(0), q2.data_ptr()
+        if w1 != 1 or ws % 16 or wp % 16:
+            weight = _aligned_rows(Nn, K, q.device).copy_(weight)
+            ws, wp = weight.stride(0), weight.data_ptr()
         if not scale.is_contiguous():
             scale = scale.contiguous()
         if not weight_scale.is_contiguous():
@@ -203,9 +214,9 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
         if bias is not None:
             bias = bias.float().contiguous()
             b = bias.data_ptr()
-        N.launch("ax_int8_gemm", dev.index, q2.data_ptr(), qs, scale.data_ptr(), weight.data_ptr(), ws, weight_scale.data_ptr(), b,
-                 out.data_ptr(), Nn, _KINDS[out_dtype], M, Nn, K, N.status_ptr(dev.index))
-    return out if q.dim() == 2 else out.view(*lead, Nn)
+        N.launch("ax_int8_gemm", index, qp, qs, scale.data_ptr(), wp, ws, weight_scale.data_ptr(), b, out.data_ptr(), Nn, kind, M, Nn, K,
+                 N.status_ptr(index))
+    return out if flat else out.view(*q.shape[:-1], Nn)
 
 
 @dataclasses.dataclass

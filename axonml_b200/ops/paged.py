@@ -65,9 +65,12 @@ def decode_attention(q, k_cache, v_cache, block_table, ctx_lens, page_size: int,
 
 
 # ------------------------------------------------------------------------------ cache in 8 bits
+_I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
+
+
 def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
-    """``(pages, Hkv, page_size, D)`` of a consistent int8 cache."""
-    if k_cache.dtype != torch.int8 or v_cache.dtype != torch.int8:
+    """``(pages, Hkv, page_size, D, GPU index or -1)`` of a consistent int8 cache."""
+    if k_cache.dtype is not _I8 or v_cache.dtype is not _I8:
         raise TypeError("the caches must be int8")
     if k_cache.dim() != 4:
         raise ValueError(f"k_cache must be [pages, Hkv, page_size, D], not {tuple(k_cache.shape)}")
@@ -78,21 +81,21 @@ def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
         raise ValueError(f"v_cache must be [pages, Hkv, page_size / 16, D, 16], not {tuple(v_cache.shape)}")
     if k_amax.shape != (pages, Hkv) or v_amax.shape != (pages, Hkv):
         raise ValueError(f"k_amax and v_amax must be [pages, Hkv] = {(pages, Hkv)}")
-    if k_amax.dtype != torch.float32 or v_amax.dtype != torch.float32:
+    if k_amax.dtype is not _F32 or v_amax.dtype is not _F32:
         raise TypeError("k_amax and v_amax must be fp32")
-    if block_table.dim() != 2 or block_table.dtype != torch.int32:
+    if block_table.dim() != 2 or block_table.dtype is not _I32:
         raise TypeError("block_table must be int32 [B, max_pages]")
     if not (k_cache.is_contiguous() and v_cache.is_contiguous() and k_amax.is_contiguous() and v_amax.is_contiguous()):
         raise ValueError("the caches and their magnitudes must be contiguous")
-    dev = k_cache.device
-    if v_cache.device != dev or k_amax.device != dev or v_amax.device != dev or block_table.device != dev:
+    dev = k_cache.get_device()
+    if v_cache.get_device() != dev or k_amax.get_device() != dev or v_amax.get_device() != dev or block_table.get_device() != dev:
         raise ValueError("the caches, their magnitudes and the block table must be on one device")
-    return pages, Hkv, P, D
+    return pages, Hkv, P, D, dev
 
 
-def _int32_vector(t, n: int, name: str, device):
-    if t.dtype != torch.int32 or t.dim() != 1 or t.shape[0] != n or t.device != device:
-        raise ValueError(f"{name} must be int32 [{n}] on {device}")
+def _int32_vector(t, n: int, name: str, index: int):
+    if t.dtype is not _I32 or t.dim() != 1 or t.shape[0] != n or t.get_device() != index:
+        raise ValueError(f"{name} must be int32 [{n}] on the cache's device")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -107,35 +110,42 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
     before is rounded to the new grid; a page written from its first slot starts anew.  ``cu_seqlens`` must not
     decrease, and two sequences of one call must not write to the same page.  On a GPU a sequence that does not fit its table or a
     page number outside the cache is skipped and reported by ``_native.check_status()``."""
-    pages, Hkv, P, D = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
-    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype != k.dtype:
+    pages, Hkv, P, D, index = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
+    if k.dim() != 3 or k.shape[1:] != (Hkv, D) or v.shape != k.shape or v.dtype is not k.dtype:
         raise ValueError(f"k and v must be [T, {Hkv}, {D}] of one type, not {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
-    if k.device != k_cache.device or v.device != k_cache.device:
+    if k.get_device() != index or v.get_device() != index:
         raise ValueError("k and v must be on the cache's device")
-    T, B = k.shape[0], block_table.shape[0]
-    starts = _int32_vector(starts, B, "starts", k.device)
+    T, (B, width) = k.shape[0], block_table.shape
+    starts = _int32_vector(starts, B, "starts", index)
+    cu = 0
     if cu_seqlens is not None:
-        cu_seqlens = _int32_vector(cu_seqlens, B + 1, "cu_seqlens", k.device)
+        cu_seqlens = _int32_vector(cu_seqlens, B + 1, "cu_seqlens", index)
+        cu = cu_seqlens.data_ptr()
     elif B == 0 or T % B:
         raise ValueError(f"without cu_seqlens, {T} tokens must divide evenly over {B} sequences")
-    if not k.is_cuda:
+    if index < 0:
         _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens)
         return
-    if k.dtype not in (torch.bfloat16, torch.float32):
+    if k.dtype is torch.bfloat16:
+        kind, vec = 1, 8
+    elif k.dtype is _F32:
+        kind, vec = 0, 4
+    else:
         raise TypeError(f"k and v must be bf16 or fp32 on a GPU, not {k.dtype}")
     if D > 512 or Hkv > 65535 or P * D > 1 << 30:
         raise ValueError(f"head_dim {D}, {Hkv} KV heads or page_size {P} are more than the kernel takes (512, 65535, 2^30 / head_dim)")
     if T == 0 or B == 0:
         return
-    vec = 16 // k.element_size()
-    if k.stride(2) != 1 or k.stride(0) % vec or k.stride(1) % vec or k.data_ptr() % 16:
+    (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
+    if k1 != 1 or kt % vec or kh % vec or k.data_ptr() % 16:
         k = k.clone(memory_format=torch.contiguous_format)
-    if v.stride(2) != 1 or v.stride(0) % vec or v.stride(1) % vec or v.data_ptr() % 16:
+        kt, kh, _ = k.stride()
+    if v1 != 1 or vt % vec or vh % vec or v.data_ptr() % 16:
         v = v.clone(memory_format=torch.contiguous_format)
+        vt, vh, _ = v.stride()
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    N.launch("ax_kv_write_int8", k.device.index, int(k.dtype == torch.bfloat16), k.data_ptr(), k.stride(0), k.stride(1), v.data_ptr(), v.stride(0),
-             v.stride(1), k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(), v_amax.data_ptr(), table.data_ptr(), starts.data_ptr(),
-             cu_seqlens.data_ptr() if cu_seqlens is not None else 0, T, B, Hkv, D, P, table.shape[1], pages, N.status_ptr(k.device.index))
+    N.launch("ax_kv_write_int8", index, kind, k.data_ptr(), kt, kh, v.data_ptr(), vt, vh, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),
+             v_amax.data_ptr(), table.data_ptr(), starts.data_ptr(), cu, T, B, Hkv, D, P, width, pages, N.status_ptr(index))
 
 
 def _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, cu_seqlens) -> None:
@@ -178,30 +188,32 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
     empty context gives zeros.  On a GPU D is 64, 128 or 256; any number of query heads per KV head.  A
     page number outside the cache and a context longer than the table are reported by
     ``_native.check_status()`` and not read."""
-    pages, Hkv, P, D = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
-    if q.dim() != 3 or q.shape[0] != block_table.shape[0] or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
-        raise ValueError(f"q must be [{block_table.shape[0]}, a multiple of {Hkv}, {D}], not {tuple(q.shape)}")
-    if q.device != k_cache.device:
+    pages, Hkv, P, D, index = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
+    B, width = block_table.shape
+    if q.dim() != 3 or q.shape[0] != B or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
+        raise ValueError(f"q must be [{B}, a multiple of {Hkv}, {D}], not {tuple(q.shape)}")
+    if q.get_device() != index:
         raise ValueError("q must be on the cache's device")
-    B, Hq, _ = q.shape
-    ctx_lens = _int32_vector(ctx_lens, B, "ctx_lens", q.device)
-    scale = scale if scale is not None else 1.0 / math.sqrt(D)
-    if not q.is_cuda:
+    Hq = q.shape[1]
+    ctx_lens = _int32_vector(ctx_lens, B, "ctx_lens", index)
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if index < 0:
         return _decode_attention_int8_cpu(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale)
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not torch.bfloat16:
         raise TypeError(f"q must be bf16 on a GPU, not {q.dtype}")
     if D not in (64, 128, 256):
         raise ValueError(f"head_dim must be 64, 128 or 256 on a GPU, not {D}")
-    q = q if q.is_contiguous() and q.data_ptr() % 16 == 0 else q.clone(memory_format=torch.contiguous_format)
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    idx, width = q.device.index, table.shape[1]
     for b0 in range(0, B, 8192):                       # the kernel keeps a running count per sequence in shared memory
         n = min(8192, B - b0)
-        ws = torch.empty(_int8_workspace(idx, n, Hq, Hkv, D, width, P), dtype=torch.float32, device=q.device)
-        N.launch("ax_decode_int8", idx, q.data_ptr() + b0 * Hq * D * 2, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),
+        ws = k_amax.new_empty(_int8_workspace(index, n, Hq, Hkv, D, width, P))
+        N.launch("ax_decode_int8", index, q.data_ptr() + b0 * Hq * D * 2, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),
                  v_amax.data_ptr(), table.data_ptr() + b0 * width * 4, ctx_lens.data_ptr() + b0 * 4, out.data_ptr() + b0 * Hq * D * 2, n, Hq, Hkv,
-                 D, P, width, pages, scale, ws.data_ptr(), N.status_ptr(idx))
+                 D, P, width, pages, scale, ws.data_ptr(), N.status_ptr(index))
     return out
 
 
