@@ -210,10 +210,11 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
     for b0 in range(0, B, 8192):                       # the kernel keeps a running count per sequence in shared memory
         n = min(8192, B - b0)
-        ws = k_amax.new_empty(_int8_workspace(index, n, Hq, Hkv, D, width, P))
+        size = _int8_workspace(index, n, Hq, Hkv, D, width, P)
+        ws = k_amax.new_empty(size) if size else None
         N.launch("ax_decode_int8", index, q.data_ptr() + b0 * Hq * D * 2, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),
                  v_amax.data_ptr(), table.data_ptr() + b0 * width * 4, ctx_lens.data_ptr() + b0 * 4, out.data_ptr() + b0 * Hq * D * 2, n, Hq, Hkv,
-                 D, P, width, pages, scale, ws.data_ptr(), N.status_ptr(index))
+                 D, P, width, pages, scale, ws.data_ptr() if size else 0, N.status_ptr(index))
     return out
 
 

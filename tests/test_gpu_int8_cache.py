@@ -88,8 +88,9 @@ def _attend(B, Hkv, G, D, P, ctx, seed=0, spare=0):
 @pytest.mark.parametrize("Hkv,G,D,P", [(8, 4, 128, 16), (1, 1, 64, 16), (2, 8, 128, 32), (3, 5, 64, 64), (2, 16, 128, 16), (1, 37, 128, 16),
                                        (2, 2, 256, 16), (1, 12, 256, 32), (4, 7, 64, 16), (16, 1, 128, 16)])
 @pytest.mark.parametrize("ctx", [[1], [16], [17], [777], [0], [0, 5, 0, 0, 300, 64, 0], [2000, 3, 1000]])
-def test_attention(Hkv, G, D, P, ctx, kernel_status):
-    got = _attend(len(ctx), Hkv, G, D, P, ctx, spare=2)
+@pytest.mark.parametrize("spare", [2, 9000])             # short tables: a cluster a head; long ones: even shares and a merge
+def test_attention(Hkv, G, D, P, ctx, spare, kernel_status):
+    got = _attend(len(ctx), Hkv, G, D, P, ctx, spare=spare)
     for b, n in enumerate(ctx):
         if n == 0:
             assert got[b].eq(0).all()
@@ -102,10 +103,13 @@ def test_attention_many_sequences_and_a_long_one(kernel_status):
     _attend(40, 8, 4, 128, 16, [int(x) for x in torch.randint(1, 2500, (40,), generator=g)], seed=5)
 
 
-def test_attention_extreme_scores_and_scales(kernel_status):
+@pytest.mark.parametrize("long_table", [False, True])
+def test_attention_extreme_scores_and_scales(long_table, kernel_status):
     """One token that takes all the weight, q rows of very different sizes, a zero q, pages of zero magnitude."""
     Hkv, G, D, P, n = 2, 4, 128, 16, 200
     table, pages = _table([(n + P - 1) // P])
+    if long_table:
+        table = torch.cat([table, torch.zeros(1, 9000, dtype=torch.int32)], 1)
     kc, vc, ka, va = R.make_cache(pages, Hkv, P, D, "cuda", seed=9)
     q = torch.randn(1, Hkv * G, D, device="cuda").bfloat16()
     q[0, 0] *= 1e4
@@ -131,13 +135,14 @@ def test_attention_extreme_scores_and_scales(kernel_status):
     assert paged.decode_attention_int8(q, kc, vc, ka, va, table.cuda(), cl16).isfinite().all()
 
 
-def test_attention_reports_bad_pages_and_contexts():
+@pytest.mark.parametrize("width", [0, 9000])
+def test_attention_reports_bad_pages_and_contexts(width):
     from axonml_b200 import _native as N
     kc, vc, ka, va = R.make_cache(4, 2, 16, 64, "cuda")
     q = torch.randn(3, 4, 64, device="cuda").bfloat16()
     cl = torch.tensor([20, 30, 9], dtype=torch.int32).cuda()
-    for table, ctx in (([[0, 1], [2, 99], [3, 0]], cl), ([[0, 1], [-1, 2], [3, 0]], cl), ([[0, 1], [2, 1], [3, 0]], cl + torch.tensor([0, 90, 0]).cuda().int())):
-        t = torch.tensor(table, dtype=torch.int32)
+    for table, ctx in (([[0, 1], [2, 99], [3, 0]], cl), ([[0, 1], [-1, 2], [3, 0]], cl), ([[0, 1], [2, 1], [3, 0]], cl + torch.tensor([0, 90 + 16 * width, 0]).cuda().int())):
+        t = torch.cat([torch.tensor(table, dtype=torch.int32), torch.zeros(3, width, dtype=torch.int32)], 1)
         got = paged.decode_attention_int8(q, kc, vc, ka, va, t.cuda(), ctx)
         with pytest.raises(N.KernelTimeout):
             N.check_status()
@@ -230,11 +235,13 @@ def test_captured_branches_memsets_and_copies(kernel_status):
             assert torch.equal(p, q)
 
 
-def test_two_calls_at_once(kernel_status):
+@pytest.mark.parametrize("long", [0, 1])
+def test_two_calls_at_once(long, kernel_status):
     """The same operators on two streams at the same time, each with its own inputs."""
     Hkv, G, D, P = 4, 4, 128, 16
     ctx = [1500, 3, 900]
     table, pages = _table([(n + P - 1) // P for n in ctx])
+    table = torch.cat([table, torch.zeros(3, 5000 * long, dtype=torch.int32)], 1)
     cl, tab = torch.tensor(ctx, dtype=torch.int32).cuda(), table.cuda()
     sets = [R.make_cache(pages, Hkv, P, D, "cuda", seed=s) + [torch.randn(3, Hkv * G, D, device="cuda").bfloat16()] for s in (1, 2)]
     alone = [paged.decode_attention_int8(c[4], *c[:4], tab, cl) for c in sets]
