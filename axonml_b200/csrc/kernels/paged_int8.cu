@@ -28,6 +28,7 @@ struct WriteArgs {
   const int* cu;              // [B + 1] first token of each row in k / v, or null: T / B tokens each
   long k_ts, k_hs, v_ts, v_hs;
   int T, B, Hkv, D, P, max_pages, num_pages;
+  int magic;                  // i * magic / 65536 is i / (D / 8) for a thread's index i (i (D / 8) < 65536)
   int* status;
 };
 
@@ -51,8 +52,8 @@ __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start,
   return (start + len - 1) / a.P - start / a.P + 1;
 }
 
-// The piece that block `slot` of the grid works on: every warp walks the rows 32 at a time, adding up
-// their pages until it passes `slot`.
+// The piece that block `slot` of the grid works on: a warp walks the rows 32 at a time, adding up their pages
+// until it passes `slot`.
 __device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& out) {
   const int lane = threadIdx.x & 31;
   int base = 0;
@@ -111,9 +112,16 @@ __global__ void __launch_bounds__(2 * kHalf, 512 / kHalf) kv_write_int8_kernel(c
   __shared__ uint32_t s_top[2 * kHalf / 32];
   chain_ready();
   chain_wait();
-  Piece pc;
-  if (!find_piece(a, (int)blockIdx.x, pc)) return;           // uniform over the block
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  __shared__ Piece s_piece;                                  // (found by one warp: the issue slots are what the kernel lacks)
+  if (warp == 0) {
+    Piece found;
+    if (!find_piece(a, (int)blockIdx.x, found)) found.count = 0;
+    if (lane == 0) s_piece = found;
+  }
+  __syncthreads();
+  const Piece pc = s_piece;
+  if (pc.count == 0) return;
   const bool is_v = threadIdx.x >= kHalf;
   const int tid = threadIdx.x & (kHalf - 1), i4 = tid & 3;
   const long ts = is_v ? a.v_ts : a.k_ts, hs = is_v ? a.v_hs : a.k_hs;
@@ -123,7 +131,7 @@ __global__ void __launch_bounds__(2 * kHalf, 512 / kHalf) kv_write_int8_kernel(c
   // K: threads side by side along a token's dims, 64 / per_row tokens at once, four of those a round.
   // V: a unit is 16 slots x 8 dims on four lanes, 16 units a round.
   const int g0 = pc.first / 16, g1 = (end + 15) / 16, units = (g1 - g0) * per_row;
-  const int across = kHalf / per_row, row0 = tid / per_row, tokens = 4 * across;
+  const int across = kHalf / per_row, row0 = (tid * a.magic) >> 16, tokens = 4 * across;
   const int rounds = is_v ? (units + kHalf / 4 - 1) / (kHalf / 4) : (pc.count + tokens - 1) / tokens;
   Raw8<T> raw[4];
   int t0, step, col = (tid - row0 * per_row) * 8, slot0 = 0;  // this thread's tokens of the round: t0, t0 + step, ...
@@ -964,7 +972,7 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   // a row of n tokens touches at most (n - 1) / P + 2 pages; a single token one
   const long rows = B < T ? B : T;
   const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
-  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, status};
+  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, (65536 + D / 8 - 1) / (D / 8), status};
   const dim3 grid((unsigned)pieces, Hkv);
   // Larger blocks shorten the latency of a big page where few blocks leave room (200 tokens, pages of 64 x 128: 6.2 us
   // against 8.4); full devices prefer the small ones (8192 tokens, pages of 16 x 128: 19.5 against 32.1).
