@@ -827,7 +827,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
 // lane), and the block's groups take the partials in turn; the largest maximum is found first, so that the
 // loads of the sums do not wait for one another.  SL = D for many heads (few blocks and few partials each),
 // 32 for few heads whose tokens went to many workers: 1 sequence of 60000 tokens and one KV head takes 20 us
-// that way, 48 with whole heads a block; 64 sequences of 777 tokens 32 us with whole heads, 41 in slices.
+// that way, 48 with whole heads a block; 300 sequences of up to 200 tokens 42 us with whole heads, 60 in slices.
 template <int D, int HG, int SL>
 __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
   constexpr int LG = SL / 4 < 32 ? SL / 4 : 32;                  // lanes of a group
@@ -1004,6 +1004,21 @@ static AttnShape attn_shape(int B, int Hq, int Hkv, int D, int max_pages, int P)
   // 777 tokens 6.2 / 8.8, 4096 11.9 / 13.1, 8192 17.8 / 15.3, 30000 50 / 24; 8 of 777 10.4 / 15.5; 64 of 777 23.8 / 31.9,
   // of up to 2048 with lengths spread over 0.3 to 1 44.7 / 44.8.
   r.cluster = 0;
+  // More heads than blocks at once: a block a head by estimated time (us, fits to full tables).  Even shares cost 9 and, a
+  // tile of a worker, 2.2 up to 14 of them, 1.55 beyond; a block a head 2.6 and, in turn, 2 and 1.6 a tile of its warps; the last
+  // turn is half full on average.  Block a head / even shares: 128 x 500 tokens, 8 KV heads 32.0 / 39.5; 300 x 200 37.8 / 45.7;
+  // 64 x 777, 32 KV heads 72.9 / 82.1; 24 x 8192, 32 KV heads 232 / 203; 64 x 16, 32 KV heads 14.9 / 11.2.
+  if (heads > most) {
+    const double turns = (double)heads / most, whole = (double)((heads + most - 1) / most);
+    const double part = per_head > kWarps ? (double)per_head / kWarps : 1.0;
+    const double block = 2.6 + 0.5 * (turns + whole) * (1.6 * part + 2.0);
+    const double shares = 9.0 + 2.2 * (chunk < 14 ? chunk : 14) + 1.55 * (chunk > 14 ? chunk - 14 : 0);
+    if (block < shares) {
+      r.cluster = 1;
+      r.blocks = (int)heads;
+      return r;
+    }
+  }
   if (heads <= most) {
     int c = 8;
     while (c > 1 && (heads * c > most || (c / 2) * kWarps >= per_head)) c /= 2;
