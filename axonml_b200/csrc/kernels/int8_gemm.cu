@@ -548,6 +548,7 @@ Choice choose(int M, int N, int K, int pairs) {
   }
   for (int bn = 16; bn <= 128; bn *= 2) {
     if (bn > 16 && M <= bn / 2) break;
+    if ((M - 1) / bn >= 65535) continue;                       // (the grid's second dimension)
     const double tiles = (double)((N + kRowsA - 1) / kRowsA) * ((M + bn - 1) / bn);
     for (int S = 1; S <= 8 && S <= (int)kb; S *= 2) {
       const double w = waves(tiles * S, slots), each = (kb + S - 1) / S;

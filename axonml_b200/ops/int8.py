@@ -15,6 +15,7 @@ import torch
 from .. import _native as N
 
 MAX_K = 131071          # 2^14 K < 2^31: the int32 sum cannot overflow
+MAX_ROWS = 1 << 30      # rows, columns and channels are 32-bit numbers on a GPU
 
 
 def _aligned_rows(rows: int, cols: int, device) -> torch.Tensor:
@@ -68,6 +69,8 @@ def _launch_rows(mode: int, x: torch.Tensor, D: int, res=None, weight=None, eps:
         x2 = _rows2d(x)
         strides = x2.stride()
     rows, dtype, index = x2.shape[0], x.dtype, x.get_device()
+    if rows > MAX_ROWS or D > MAX_ROWS:
+        raise ValueError(f"{rows} rows of {D} are more than the kernel takes ({MAX_ROWS})")
     wk = kind = _kind(dtype, "x")
     if D % 16 == 0 and mode != 2 and strides[0] == D:
         q = torch.empty_like(x2, dtype=_I8)
@@ -195,6 +198,8 @@ def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weig
         y = (q2.double() @ weight.double().t()).float() * scale.reshape(-1, 1) * weight_scale
         y = y if bias is None else y + bias.float()
         return y.to(out_dtype).view(*q.shape[:-1], Nn)
+    if M > MAX_ROWS or Nn > MAX_ROWS:
+        raise ValueError(f"{M} rows and {Nn} channels are more than the kernel takes ({MAX_ROWS})")
     out = torch.empty_strided((M, Nn), (Nn, 1), dtype=out_dtype, device=q.device)
     if M and Nn:
         qs, q1 = q2.stride()

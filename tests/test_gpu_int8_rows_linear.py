@@ -168,3 +168,23 @@ def test_int8_operators_in_a_graph_and_on_another_stream(kernel_status):
 def test_gpu_refusals(call, err):
     with pytest.raises(err):
         call()
+
+
+def test_int8_linear_of_very_many_rows(kernel_status):
+    """More row blocks than a grid's second dimension holds."""
+    M, K, Nn = 8_400_000, 4096, 16
+    q = torch.randint(-127, 128, (1, K), dtype=torch.int8, device="cuda")
+    w = torch.randint(-127, 128, (Nn, K), dtype=torch.int8, device="cuda")
+    s, ws = torch.ones(M, device="cuda"), torch.ones(Nn, device="cuda")
+    y = I.int8_linear(q.expand(M, K), s, w, ws, out_dtype=torch.float32)
+    assert y.eq((q.double() @ w.double().t()).float()).all()
+
+
+def test_more_rows_than_the_kernels_take_are_refused():
+    x = torch.zeros(1, 16, device="cuda").expand(I.MAX_ROWS + 1, 16)
+    with pytest.raises(ValueError):
+        I.quantize_int8(x)
+    q = torch.zeros(1, 16, dtype=torch.int8, device="cuda").expand(I.MAX_ROWS + 1, 16)
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(ValueError):
+        I.int8_linear(q, one.expand(I.MAX_ROWS + 1), q[:1], one)
