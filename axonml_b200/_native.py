@@ -169,8 +169,7 @@ def status_word(device=None) -> torch.Tensor:
     key = (dev.type, dev.index)
     t = _STATUS.get(key)
     if t is None:
-        t = torch.zeros(4, dtype=torch.int32, device=dev)
-        _STATUS[key] = t
+        t = _STATUS.setdefault(key, torch.zeros(4, dtype=torch.int32, device=dev))    # (one word, also for threads in a race)
     return t
 
 

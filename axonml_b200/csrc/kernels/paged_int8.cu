@@ -28,6 +28,7 @@ struct WriteArgs {
   const int* cu;              // [B + 1] first token of each row in k / v, or null: T / B tokens each
   long k_ts, k_hs, v_ts, v_hs;
   int T, B, Hkv, D, P, max_pages, num_pages;
+  int per_row;                // blocks of a row without cu
   int magic;                  // i * magic / 65536 is i / (D / 8) for a thread's index i (i (D / 8) < 65536)
   int* status;
 };
@@ -52,39 +53,44 @@ __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start,
   return (start + len - 1) / a.P - start / a.P + 1;
 }
 
-// The piece that block `slot` of the grid works on: a warp walks the rows 32 at a time, adding up their pages
-// until it passes `slot`.
+// The piece that block `slot` of the grid works on.  n tokens touch at most (n + 2 P - 2) / P pages, so row b's slots begin
+// at (cu[b] + b (2 P - 2)) / P: a warp looks for the row 128 at a time, and slots past a row's pages have nothing to do.
+// (Counting pages row by row instead took 568 us for a token of each of 2048 sequences with 8 heads, 8140 for 8192.)
 __device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& out) {
-  const int lane = threadIdx.x & 31;
-  int base = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    int start = 0, src = 0, len = 0, n = 0;
-    if (b0 + lane < a.B) n = row_pieces(a, b0 + lane, start, src, len);
-    int upto = n;
+  int b = 0, start, src, len, j;
+  if (a.cu == nullptr) {
+    b = slot / a.per_row;
+    j = slot - b * a.per_row;
+  } else {
+    const int lane = threadIdx.x & 31;
+    auto at = [&](int r) { return (long)min(max(a.cu[r], 0), a.T) + (long)r * (2 * a.P - 2); };
+    const long below = ((long)slot + 1) * a.P;
+    for (int n = a.B;;) {                                    // the row is one of n from b on
+      const int step = (n + 127) / 128;
+      int count = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, upto, o);
-      if (lane >= o) upto += t;
+      for (int k = 0; k < 4; ++k) {
+        const int i = (k * 32 + lane) * step;
+        count += __popc(__ballot_sync(0xffffffffu, i < n && at(b + i) < below));
+      }
+      const int skip = max(count - 1, 0) * step;
+      b += skip;
+      if (step == 1) break;
+      n = min(step, n - skip);
     }
-    const int total = __shfl_sync(0xffffffffu, upto, 31);
-    if (slot < base + total) {
-      const int own = __ffs(__ballot_sync(0xffffffffu, base + upto > slot)) - 1;
-      const int j = slot - base - (__shfl_sync(0xffffffffu, upto - n, own));
-      start = __shfl_sync(0xffffffffu, start, own);
-      src = __shfl_sync(0xffffffffu, src, own);
-      len = __shfl_sync(0xffffffffu, len, own);
-      const int idx = start / a.P + j;                       // which page of the row
-      const int lo = max(start, idx * a.P), hi = min(start + len, (idx + 1) * a.P);
-      out.page = a.table[(long)(b0 + own) * a.max_pages + idx];
-      out.first = lo - idx * a.P;
-      out.count = hi - lo;
-      out.src = src + lo - start;
-      if (out.page < 0 || out.page >= a.num_pages) { set_status(a.status, kBadArgument, 1201); return false; }
-      return true;
-    }
-    base += total;
+    const long x = at(b);
+    j = slot - (x <= 0x7fffffffL ? (int)x / a.P : (int)(x / a.P));
   }
-  return false;
+  const int pages = row_pieces(a, b, start, src, len);
+  if (j < 0 || j >= pages) return false;
+  const int idx = start / a.P + j, page0 = idx * a.P;        // which page of the row
+  const int lo = max(start, page0), n = min(start + len - page0, a.P) + page0 - lo;
+  out.page = a.table[(long)b * a.max_pages + idx];
+  out.first = lo - page0;
+  out.count = n;
+  out.src = src + lo - start;
+  if (out.page < 0 || out.page >= a.num_pages) { set_status(a.status, kBadArgument, 1201); return false; }
+  return true;
 }
 
 // rint(q a_old / a_new) of four bytes
@@ -290,6 +296,7 @@ struct AttnArgs {
   float* part;                 // [workers][2][HG][D]
   float* ml;                   // [workers][2][HG][2]
   int B, Hq, Hkv, G, nblk, P, max_pages, num_pages, min_chunk, workers;
+  int* seen;                   // [B + 1] tiles of the sequences before, for the merge
   int cluster;                 // ONE: blocks that share a head
   float scale_log2;            // scale * log2(e) / 127
   int* status;
@@ -357,7 +364,7 @@ struct AttnCfg {
   static constexpr int kBlocks = D == 256 ? 2 : 4;               // blocks per SM that registers and shared memory allow
 };
 constexpr float kSlack = 8.f;                                    // log2 of the largest weight
-constexpr float kNone = -1e30f;                                  // running maximum before the first score
+constexpr float kNone = -3.402823466e38f;                        // running maximum before the first score (-FLT_MAX: not above a finite one)
 constexpr float kFaint = 1.f / 8.f;
 
 // NB: blocks of eight query heads.
@@ -411,6 +418,8 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
       if (lane == 0) prefix[0] = 0;
     }
     __syncthreads();
+    if (blockIdx.x == 0)
+      for (int i = threadIdx.x; i <= a.B; i += kWarps * 32) a.seen[i] = prefix[i];
     const int total = prefix[a.B] * VH, chunk = chunk_of(a, total);
     w = warp * (int)gridDim.x + (int)blockIdx.x;                 // neighbouring workers on different SMs
     const long first = (long)w * chunk;
@@ -828,31 +837,26 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
 // loads of the sums do not wait for one another.  SL = D for many heads (few blocks and few partials each),
 // 32 for few heads whose tokens went to many workers: 1 sequence of 60000 tokens and one KV head takes 20 us
 // that way, 48 with whole heads a block; 300 sequences of up to 200 tokens 42 us with whole heads, 60 in slices.
-template <int D, int HG, int SL>
-__global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
+// HP: heads of a block, a warp each (1: the whole block works on one).  Most heads of a large batch lie in one worker's share and
+// need nothing: 8000 sequences of 500 tokens, 32 query heads, take 1646 us with eight heads a block, 1696 with one.
+template <int D, int HG, int SL, int HP>
+__global__ void __launch_bounds__(SL == 32 ? 1024 : 256) merge_int8_kernel(const AttnArgs a) {
   constexpr int LG = SL / 4 < 32 ? SL / 4 : 32;                  // lanes of a group
   constexpr int NV = SL / 4 / LG;                                // float4s of a lane
   constexpr int GW = 32 / LG;                                    // groups of a warp
   __shared__ float s_top[32], s_sum[32];
   __shared__ float4 s_acc[SL == 32 ? 32 : 8][SL / 4];            // [warps]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-  const int b = blockIdx.x / a.Hq, hq = blockIdx.x % a.Hq;
+  const int lane = threadIdx.x & 31, warp = HP > 1 ? 0 : threadIdx.x >> 5, warps = HP > 1 ? 1 : blockDim.x >> 5;
+  const int tid = warp * 32 + lane, threads = warps * 32;
+  const int item = blockIdx.x * HP + (HP > 1 ? threadIdx.x >> 5 : 0), b = item / a.Hq, hq = item - b * a.Hq;
   const int h = hq / a.G, hg = hq % a.G, vh = h * a.nblk + hg / HG, row = hg % HG;
   const int VH = a.Hkv * a.nblk;
   chain_wait();
-  int before = 0, total = 0, tb = 0;
-  for (int b0 = 0; b0 < a.B; b0 += 32) {
-    const int n = b0 + lane < a.B ? tiles_of(a, b0 + lane) : 0;
-    total += n;
-    if (b0 + lane < b) before += n;
-    if (b0 + lane == b) tb = n;
-  }
-  before = __reduce_add_sync(0xffffffffu, before);
-  total = __reduce_add_sync(0xffffffffu, total);
-  tb = __reduce_add_sync(0xffffffffu, tb);
+  if (HP > 1 && b >= a.B) return;
+  const int before = a.seen[b], tb = a.seen[b + 1] - before, total = a.seen[a.B];
   __nv_bfloat16* op = a.out + ((long)b * a.Hq + hq) * D + blockIdx.y * SL;
   if (tb == 0) {
-    for (int d = threadIdx.x; d < SL; d += blockDim.x) op[d] = __float2bfloat16(0.f);
+    for (int d = tid; d < SL; d += threads) op[d] = __float2bfloat16(0.f);
     return;
   }
   const int chunk = chunk_of(a, total * VH), seg = before * VH + vh * tb;
@@ -860,7 +864,7 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
   if (pieces == 1) return;                                       // one worker had it all and wrote it
   auto slot_of = [&](int i) { return ((long)(w0 + i) * 2 + (i == 0 ? 1 : 0)) * HG + row; };
   float M = -INFINITY;
-  for (int i = threadIdx.x; i < pieces; i += blockDim.x) M = fmaxf(M, a.ml[slot_of(i) * 2]);
+  for (int i = tid; i < pieces; i += threads) M = fmaxf(M, a.ml[slot_of(i) * 2]);
   M = warp_max(M);
   if (warps > 1) {
     if (lane == 0) s_top[warp] = M;
@@ -924,16 +928,20 @@ __global__ void __launch_bounds__(1024) merge_int8_kernel(const AttnArgs a) {
           make_uint2(pack_bf16x2(acc[k].x * inv, acc[k].y * inv), pack_bf16x2(acc[k].z * inv, acc[k].w * inv));
 }
 
+// Sequences of a launch: their running counts lie in shared memory, where four blocks an SM leave 4 KB each (2048 of 2048
+// tokens, 8 KV heads: 1826 us in one launch with three blocks an SM, 1429 in two).
+constexpr int kMaxSeqs = 1024;
 template <int D, int HG, bool ONE>
 int launch_decode(const AttnArgs& a, int blocks, int smem, cudaStream_t stream) {
   auto kern = decode_int8_kernel<D, HG / 8, ONE>;
-  static int configured[64] = {0};
+  static bool configured[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
-  if (dev < 0 || dev >= 64 || configured[dev] < smem) {
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev < 0 || dev >= 64 || !configured[dev]) {                // the most that any call takes: host threads in a race set the same
+    const int most = ONE ? smem : smem + (kMaxSeqs - a.B) * 4;
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
     if (e != cudaSuccess) return (int)e;
-    if (dev >= 0 && dev < 64) configured[dev] = smem;
+    if (dev >= 0 && dev < 64) configured[dev] = true;
   }
   return axh::launch_chained(kern, dim3(blocks), dim3(kWarps * 32), smem, ONE ? a.cluster : 1, stream, a);
 }
@@ -950,10 +958,11 @@ int launch_attn(const AttnArgs& a, int blocks, cudaStream_t stream) {
   int warps = 1;
   if ((long)a.B * a.Hq >= 4 * axh::sm_count()) {
     while (warps < 8 && warps * 2 < per) warps *= 2;
-    return axh::launch_chained(merge_int8_kernel<D, HG, D>, dim3(a.B * a.Hq), dim3(32 * warps), 0, 1, stream, a);
+    if (warps == 1) return axh::launch_chained(merge_int8_kernel<D, HG, D, 8>, dim3((a.B * a.Hq + 7) / 8), dim3(256), 0, 1, stream, a);
+    return axh::launch_chained(merge_int8_kernel<D, HG, D, 1>, dim3(a.B * a.Hq), dim3(32 * warps), 0, 1, stream, a);
   }
   while (warps < 32 && warps * 4 < per) warps *= 2;
-  return axh::launch_chained(merge_int8_kernel<D, HG, 32>, dim3(a.B * a.Hq, D / 32), dim3(32 * warps), 0, 1, stream, a);
+  return axh::launch_chained(merge_int8_kernel<D, HG, 32, 1>, dim3(a.B * a.Hq, D / 32), dim3(32 * warps), 0, 1, stream, a);
 }
 
 }  // namespace
@@ -969,10 +978,11 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   if (D % 16 || D > 512 || P % 16 || P <= 0 || (long)P * D > (1L << 30) || Hkv > 65535 || (cu == nullptr && T % B)) return -1;
   const int vec = dt == 1 ? 8 : 4;
   if ((k_ts % vec) || (k_hs % vec) || (v_ts % vec) || (v_hs % vec) || (((uintptr_t)k | (uintptr_t)v | (uintptr_t)kc | (uintptr_t)vc) & 15)) return -2;
-  // a row of n tokens touches at most (n - 1) / P + 2 pages; a single token one
-  const long rows = B < T ? B : T;
-  const long pieces = (cu == nullptr && T == B) ? B : T / P + 2 * rows;
-  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, (65536 + D / 8 - 1) / (D / 8), status};
+  // a row of n tokens touches at most (n + 2 P - 2) / P pages; a single token one
+  const int per_row = T == B ? 1 : (int)((T / B + 2L * P - 2) / P);
+  const long pieces = cu == nullptr ? (long)B * per_row : (T + B * (2L * P - 2)) / P + 1;
+  if (pieces > 0x7fffffffL) return -3;
+  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, per_row, (65536 + D / 8 - 1) / (D / 8), status};
   const dim3 grid((unsigned)pieces, Hkv);
   // Larger blocks shorten the latency of a big page where few blocks leave room (200 tokens, pages of 64 x 128: 6.2 us
   // against 8.4); full devices prefer the small ones (8192 tokens, pages of 16 x 128: 19.5 against 32.1).
@@ -1042,7 +1052,7 @@ static AttnShape attn_shape(int B, int Hq, int Hkv, int D, int max_pages, int P)
 AX_API long ax_decode_int8_workspace(int B, int Hq, int Hkv, int D, int max_pages, int P) {
   if (Hkv <= 0 || Hq % Hkv || P <= 0) return 0;
   const AttnShape r = attn_shape(B, Hq, Hkv, D, max_pages, P);
-  return r.cluster ? 0 : (long)r.blocks * kWarps * 2 * r.HG * (D + 2);
+  return r.cluster ? 0 : (long)r.blocks * kWarps * 2 * r.HG * (D + 2) + B + 1;
 }
 
 // out[B, Hq, D] = attention of q[B, Hq, D] (bf16, contiguous) over the first ctx[b] tokens of each sequence.
@@ -1052,13 +1062,14 @@ AX_API int ax_decode_int8(const void* q, const int8_t* kc, const int8_t* vc, con
                           const int* ctx, void* out, int B, int Hq, int Hkv, int D, int P, int max_pages, int num_pages, float scale,
                           float* workspace, int* status, cudaStream_t stream) {
   if (B <= 0) return 0;
-  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || P <= 0 || P % 16 || B > 8192 || (long)B * Hq > 0x7fffffffL) return -1;
+  if (Hkv <= 0 || Hq <= 0 || Hq % Hkv || P <= 0 || P % 16 || B > kMaxSeqs || (long)B * Hq > 0x7fffffffL) return -1;
   if (((uintptr_t)q | (uintptr_t)kc | (uintptr_t)vc | (uintptr_t)out | (uintptr_t)workspace) & 15) return -2;
   const AttnShape r = attn_shape(B, Hq, Hkv, D, max_pages, P);
   const int HG = r.HG, blocks = r.blocks, workers = blocks * kWarps;
-  if ((long)B * Hkv * r.nblk * ((long)max_pages * P / kTile) > 0x7fffffffL || (long)num_pages * Hkv * (P / kTile) > 0x7fffffffL) return -3;
+  // flat tiles and the end of a share are ints
+  if ((long)B * Hkv * r.nblk * ((long)max_pages * P / kTile) > 0x7f000000L || (long)num_pages * Hkv * (P / kTile) > 0x7fffffffL) return -3;
   AttnArgs a{(const __nv_bfloat16*)q, kc, vc, ka, va, table, ctx, (__nv_bfloat16*)out, workspace, workspace + (long)workers * 2 * HG * D,
-             B, Hq, Hkv, Hq / Hkv, r.nblk, P, max_pages, num_pages, r.min_chunk, workers, r.cluster, scale * 1.4426950408889634f / 127.f, status};
+             B, Hq, Hkv, Hq / Hkv, r.nblk, P, max_pages, num_pages, r.min_chunk, workers, (int*)(workspace + (long)workers * 2 * HG * (D + 2)), r.cluster, scale * 1.4426950408889634f / 127.f, status};
 #define AX_ATTN(DD)                                                      \
   return HG == 8 ? launch_attn<DD, 8>(a, blocks, stream) : launch_attn<DD, 16>(a, blocks, stream)
   switch (D) {

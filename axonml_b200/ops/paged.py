@@ -9,7 +9,7 @@ import math
 import torch
 
 from .. import _native as N
-from .int8 import TINY
+from .int8 import MAX_ROWS, TINY, _no_gradient
 
 
 def kv_write(k, v, k_cache, v_cache, block_table, seq_ids, positions, page_size: int) -> None:
@@ -75,8 +75,8 @@ def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
     if k_cache.dim() != 4:
         raise ValueError(f"k_cache must be [pages, Hkv, page_size, D], not {tuple(k_cache.shape)}")
     pages, Hkv, P, D = k_cache.shape
-    if P % 16 or P == 0 or D % 16 or D == 0:
-        raise ValueError(f"page_size {P} and head_dim {D} must be multiples of 16")
+    if P % 16 or P == 0 or D % 16 or D == 0 or Hkv == 0:
+        raise ValueError(f"page_size {P} and head_dim {D} must be multiples of 16, and {Hkv} KV heads not none")
     if v_cache.shape != (pages, Hkv, P // 16, D, 16):
         raise ValueError(f"v_cache must be [pages, Hkv, page_size / 16, D, 16], not {tuple(v_cache.shape)}")
     if k_amax.shape != (pages, Hkv) or v_amax.shape != (pages, Hkv):
@@ -115,6 +115,8 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
         raise ValueError(f"k and v must be [T, {Hkv}, {D}] of one type, not {tuple(k.shape)} {k.dtype}, {tuple(v.shape)} {v.dtype}")
     if k.get_device() != index or v.get_device() != index:
         raise ValueError("k and v must be on the cache's device")
+    if k.requires_grad or v.requires_grad:
+        _no_gradient()
     T, (B, width) = k.shape[0], block_table.shape
     starts = _int32_vector(starts, B, "starts", index)
     cu = 0
@@ -132,8 +134,8 @@ def kv_write_int8(k, v, k_cache, v_cache, k_amax, v_amax, block_table, starts, c
         kind, vec = 0, 4
     else:
         raise TypeError(f"k and v must be bf16 or fp32 on a GPU, not {k.dtype}")
-    if D > 512 or Hkv > 65535 or P * D > 1 << 30:
-        raise ValueError(f"head_dim {D}, {Hkv} KV heads or page_size {P} are more than the kernel takes (512, 65535, 2^30 / head_dim)")
+    if D > 512 or Hkv > 65535 or P * D > 1 << 30 or T > MAX_ROWS:
+        raise ValueError(f"head_dim {D}, {Hkv} KV heads, page_size {P} or {T} tokens are more than the kernel takes (512, 65535, 2^30 / head_dim, {MAX_ROWS})")
     if T == 0 or B == 0:
         return
     (kt, kh, k1), (vt, vh, v1) = k.stride(), v.stride()
@@ -194,6 +196,8 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
         raise ValueError(f"q must be [{B}, a multiple of {Hkv}, {D}], not {tuple(q.shape)}")
     if q.get_device() != index:
         raise ValueError("q must be on the cache's device")
+    if q.requires_grad:
+        _no_gradient()
     Hq = q.shape[1]
     ctx_lens = _int32_vector(ctx_lens, B, "ctx_lens", index)
     if scale is None:
@@ -208,8 +212,9 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    for b0 in range(0, B, 8192):                       # the kernel keeps a running count per sequence in shared memory
-        n = min(8192, B - b0)
+    each = B if B <= 1024 else -(-B // -(-B // 1024))  # the kernel keeps a running count per sequence in shared memory
+    for b0 in range(0, B, each or 1):
+        n = min(each, B - b0)
         size = _int8_workspace(index, n, Hq, Hkv, D, width, P)
         ws = k_amax.new_empty(size) if size else None
         N.launch("ax_decode_int8", index, q.data_ptr() + b0 * Hq * D * 2, k_cache.data_ptr(), v_cache.data_ptr(), k_amax.data_ptr(),

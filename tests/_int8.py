@@ -154,3 +154,23 @@ class Recorder:
         q, kc, vc, ka, va, table, ctx = a[:7]
         want, off = attention(q, kc, v_rows(vc), ka, va, table.tolist(), ctx.tolist(), default_scale(q.shape[-1]))
         assert ((got.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
+
+
+def far_below(n, ctx, device):
+    """A cache whose keys are all alike, a query that scores each -1.1e32, and what attention gives: the mean of the values."""
+    B, D, P = len(ctx), 128, 16
+    per = (n + P - 1) // P
+    kc, vc, ka, va = make_cache(B * per, 1, P, D, device, seed=5)
+    kc.fill_(127)
+    ka.fill_(1e31)
+    table = torch.arange(B * per, dtype=torch.int32, device=device).view(B, per)
+    q = torch.full((B, 2, D), -1.0, dtype=torch.bfloat16, device=device)
+    rows = v_rows(vc).double() * (va.double() / 127)[..., None, None]
+    want = torch.stack([rows[table[b].long(), 0].reshape(-1, D)[:c].mean(0).expand(2, D) for b, c in enumerate(ctx)])
+    return [kc, vc, ka, va], q, table, want
+
+
+def far_below_off(want, dtype):
+    """Equal scores: weights of one and a sum that is exact; the weights times a page's magnitude ratio are rounded to fp16
+    (2^-11 of the values, whose mean of magnitudes is below 8 here), the result to its type."""
+    return 2.0 ** -11 * 8 + torch.finfo(dtype).eps / 2 * (want.abs() + 2.0 ** -8)

@@ -312,3 +312,112 @@ def test_engine_in_eight_bits(weights, kv, kernel_status, monkeypatch):
     assert all(len(x) == 24 for x in a + b)
     if weights:                                           # the Q4_K product adds split sums in no fixed order, the int8 one is exact
         assert a == b
+
+
+@pytest.mark.parametrize("n,ctx", [(1, [1]), (40, [40, 17]), (700, [700, 16, 333])])
+@pytest.mark.parametrize("spare", [0, 9000])
+def test_attention_of_scores_far_below_zero(n, ctx, spare, kernel_status):
+    c, q, table, want = R.far_below(n, ctx, "cuda")
+    table = torch.cat([table, torch.zeros(len(ctx), spare, dtype=torch.int32, device="cuda")], 1)
+    got = paged.decode_attention_int8(q, *c, table, torch.tensor(ctx, dtype=torch.int32).cuda())
+    assert ((got.double() - want).abs() <= R.far_below_off(want, q.dtype)).all()
+
+
+def test_write_at_the_largest_positions(kernel_status):
+    """The last page ends at position 2^31: all but its last slot can be written."""
+    P, width = 1 << 20, 2048
+    table = torch.zeros(1, width, dtype=torch.int32)
+    k, v = torch.randn(16, 1, 16).bfloat16(), torch.randn(16, 1, 16).bfloat16()
+    cpu = R.make_cache(1, 1, P, 16, "cpu", seed=2)
+    gpu = [t.cuda() for t in cpu]
+    st = torch.tensor([2 ** 31 - 17], dtype=torch.int32)
+    paged.kv_write_int8(k, v, *cpu, table, st)
+    paged.kv_write_int8(k.cuda(), v.cuda(), *gpu, table.cuda(), st.cuda())
+    for a, b in zip(gpu, cpu):
+        assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("B", [1, 33, 2000])
+def test_write_of_one_token_each_with_bad_rows(B):
+    """Without offsets a token's page is its row's: a bad row leaves the others alone."""
+    from axonml_b200 import _native as N
+    Hkv, P, D = 2, 16, 64
+    k, v = torch.randn(B, Hkv, D, device="cuda").bfloat16(), torch.randn(B, Hkv, D, device="cuda").bfloat16()
+    gpu = R.make_cache(B, Hkv, P, D, "cuda", seed=4)
+    st = torch.arange(B, dtype=torch.int32) % 16
+    st[0] = -1
+    want = [t.cpu() for t in gpu]
+    table = torch.arange(B, dtype=torch.int32)[:, None]
+    paged.kv_write_int8(k, v, *gpu, table.cuda(), st.cuda())
+    with pytest.raises(N.KernelTimeout):
+        N.check_status()
+    if B > 1:
+        paged.kv_write_int8(k[1:].cpu(), v[1:].cpu(), *want, table[1:], st[1:])
+    for a, b in zip(gpu, want):
+        assert torch.equal(a.cpu(), b)
+
+
+def test_too_many_tokens_are_refused():
+    c = R.make_cache(1, 1, 16, 64, "cuda")
+    k = torch.zeros(1, 1, 64, device="cuda").bfloat16().expand((1 << 30) + 1, 1, 64)
+    with pytest.raises(ValueError):
+        paged.kv_write_int8(k, k, *c, torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"))
+
+
+def test_attention_from_several_threads(kernel_status):
+    """Batches of very different size from host threads at the same time."""
+    import threading
+    cases = []
+    for i, B in enumerate((1, 3000, 40, 8000)):
+        c = R.make_cache(B, 1, 16, 64, "cuda", seed=i)
+        q = torch.randn(B, 1, 64, device="cuda").bfloat16()
+        table = torch.cat([torch.arange(B, dtype=torch.int32)[:, None], torch.zeros(B, 600, dtype=torch.int32)], 1).cuda()
+        cl = (torch.arange(B, dtype=torch.int32) % 17).cuda()
+        cases.append((q, *c, table, cl))
+    torch.cuda.synchronize()
+    got, errors = [[] for _ in cases], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got[i].append(paged.decode_attention_int8(*cases[i]))
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:
+            errors.append(e)
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(cases))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors
+    for a, x in zip(cases, got):
+        alone = paged.decode_attention_int8(*a)
+        assert len(x) == 10 and all(torch.equal(y, alone) for y in x)
+
+
+@pytest.mark.parametrize("B,spare", [(1024, 0), (1025, 700), (2500, 0), (2500, 700)])
+def test_attention_of_very_many_sequences(B, spare, kernel_status):
+    g = torch.Generator().manual_seed(B)
+    _attend(B, 1, 4, 64, 16, [int(x) for x in torch.randint(0, 60, (B,), generator=g)], seed=6, spare=spare)
+
+
+@pytest.mark.parametrize("B", [129, 2000])
+def test_write_of_very_many_sequences(B, kernel_status):
+    """Rows of zero, one and more tokens, found by a search over the offsets."""
+    Hkv, P, D = 1, 16, 64
+    g = torch.Generator().manual_seed(B)
+    lens = [int(x) for x in torch.tensor([0, 0, 1, 1, 2, 40])[torch.randint(0, 6, (B,), generator=g)]]
+    starts = [int(x) for x in torch.randint(0, 33, (B,), generator=g)]
+    table, pages = _table([(s + n + P - 1) // P for s, n in zip(starts, lens)])
+    first = 3                                              # rows before the first sequence are ignored too
+    T = first + sum(lens) + 2
+    k, v = torch.randn(T, Hkv, D).bfloat16(), torch.randn(T, Hkv, D).bfloat16()
+    cu = first + torch.tensor([0] + lens).cumsum(0).to(torch.int32)
+    cpu = R.make_cache(pages, Hkv, P, D, "cpu")
+    gpu = [t.cuda() for t in cpu]
+    st = torch.tensor(starts, dtype=torch.int32)
+    paged.kv_write_int8(k, v, *cpu, table, st, cu.int())
+    paged.kv_write_int8(k.cuda(), v.cuda(), *gpu, table.cuda(), st.cuda(), cu.int().cuda())
+    for a, b in zip(gpu, cpu):
+        assert torch.equal(a.cpu(), b)

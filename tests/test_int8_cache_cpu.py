@@ -104,3 +104,26 @@ def test_attention_refusals(change, err):
         a[name] = f(a[name])
     with pytest.raises(err):
         paged.decode_attention_int8(**a)
+
+
+def test_no_gradients_and_no_heads():
+    a = _good()
+    with pytest.raises(RuntimeError):
+        paged.kv_write_int8(**{**a, "k": a["k"].float().requires_grad_(), "v": a["v"].float()})
+    caches = {n: a[n] for n in ("k_cache", "v_cache", "k_amax", "v_amax", "block_table")}
+    q, cl = torch.randn(2, 4, 16, requires_grad=True), torch.tensor([3, 6], dtype=torch.int32)
+    with pytest.raises(RuntimeError):
+        paged.decode_attention_int8(q, **caches, ctx_lens=cl)
+    with torch.no_grad():
+        paged.decode_attention_int8(q, **caches, ctx_lens=cl)
+    none = R.make_cache(2, 0, 16, 16, "cpu")
+    with pytest.raises(ValueError):
+        paged.decode_attention_int8(q.detach(), *none, a["block_table"], cl)
+
+
+@pytest.mark.parametrize("n,ctx", [(1, [1]), (40, [40, 17])])
+def test_attention_of_scores_far_below_zero(n, ctx):
+    """Scores near -1e32: the weights are those of the differences."""
+    c, q, table, want = R.far_below(n, ctx, "cpu")
+    got = paged.decode_attention_int8(q, *c, table, torch.tensor(ctx, dtype=torch.int32))
+    assert ((got.double() - want).abs() <= R.far_below_off(want, q.dtype)).all()
