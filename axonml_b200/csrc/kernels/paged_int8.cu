@@ -28,12 +28,17 @@ struct WriteArgs {
   const int* cu;              // [B + 1] first token of each row in k / v, or null: T / B tokens each
   long k_ts, k_hs, v_ts, v_hs;
   int T, B, Hkv, D, P, max_pages, num_pages;
-  int per_row;                // blocks of a row without cu
+  int per_row, each;          // blocks and tokens of a row without cu
+  int shift;                  // log2(P), or -1 where P is no power of two
   int magic;                  // i * magic / 65536 is i / (D / 8) for a thread's index i (i (D / 8) < 65536)
   int* status;
 };
 
 struct Piece { int page, first, count, src; };   // slots [first, first + count) of a page, from token src
+
+// x / P.  A block waits for a chain of these and of loads before its first value arrives.
+template <typename I>
+__device__ __forceinline__ int page_of(const WriteArgs& a, I x) { return (int)(a.shift >= 0 ? x >> a.shift : x / a.P); }
 
 // Pages touched by row b: 0 for an empty row or one that does not fit.
 __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start, int& src, int& len) {
@@ -42,7 +47,7 @@ __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start,
     src = a.cu[b];
     len = a.cu[b + 1] - src;
   } else {
-    len = a.T / a.B;
+    len = a.each;
     src = b * len;
   }
   if (len <= 0) return 0;
@@ -50,40 +55,55 @@ __device__ __forceinline__ int row_pieces(const WriteArgs& a, int b, int& start,
     set_status(a.status, kBadArgument, 1200);
     return 0;
   }
-  return (start + len - 1) / a.P - start / a.P + 1;
+  return page_of(a, start + len - 1) - page_of(a, start) + 1;
 }
 
 // The piece that block `slot` of the grid works on.  n tokens touch at most (n + 2 P - 2) / P pages, so row b's slots begin
 // at (cu[b] + b (2 P - 2)) / P: a warp looks for the row 128 at a time, and slots past a row's pages have nothing to do.
-// (Counting pages row by row instead took 568 us for a token of each of 2048 sequences with 8 heads, 8140 for 8192.)
+// (A token of each of 2048 sequences, 8 heads: 79 us; 568 when a warp counted the pages of the rows before.)
 __device__ __forceinline__ bool find_piece(const WriteArgs& a, int slot, Piece& out) {
-  int b = 0, start, src, len, j;
+  int b = 0, start = 0, src = 0, len = 0, j, pages;
   if (a.cu == nullptr) {
-    b = slot / a.per_row;
+    b = a.per_row == 1 ? slot : slot / a.per_row;
     j = slot - b * a.per_row;
+    pages = row_pieces(a, b, start, src, len);
   } else {
     const int lane = threadIdx.x & 31;
     auto at = [&](int r) { return (long)min(max(a.cu[r], 0), a.T) + (long)r * (2 * a.P - 2); };
     const long below = ((long)slot + 1) * a.P;
-    for (int n = a.B;;) {                                    // the row is one of n from b on
-      const int step = (n + 127) / 128;
-      int count = 0;
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int i = (k * 32 + lane) * step;
-        count += __popc(__ballot_sync(0xffffffffu, i < n && at(b + i) < below));
+    if (a.B <= 32) {                                         // a lane a row
+      long x = below;
+      pages = 0;
+      if (lane < a.B) {
+        x = at(lane);
+        pages = row_pieces(a, lane, start, src, len);
       }
-      const int skip = max(count - 1, 0) * step;
-      b += skip;
-      if (step == 1) break;
-      n = min(step, n - skip);
+      b = max(__popc(__ballot_sync(0xffffffffu, x < below)) - 1, 0);
+      j = slot - __shfl_sync(0xffffffffu, page_of(a, x), b);
+      pages = __shfl_sync(0xffffffffu, pages, b);
+      start = __shfl_sync(0xffffffffu, start, b);
+      src = __shfl_sync(0xffffffffu, src, b);
+      len = __shfl_sync(0xffffffffu, len, b);
+    } else {
+      for (int n = a.B;;) {                                    // the row is one of n from b on
+        const int step = (n + 127) / 128;
+        int count = 0;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int i = (k * 32 + lane) * step;
+          count += __popc(__ballot_sync(0xffffffffu, i < n && at(b + i) < below));
+        }
+        const int skip = max(count - 1, 0) * step;
+        b += skip;
+        if (step == 1) break;
+        n = min(step, n - skip);
+      }
+      j = slot - page_of(a, at(b));
+      pages = row_pieces(a, b, start, src, len);
     }
-    const long x = at(b);
-    j = slot - (x <= 0x7fffffffL ? (int)x / a.P : (int)(x / a.P));
   }
-  const int pages = row_pieces(a, b, start, src, len);
   if (j < 0 || j >= pages) return false;
-  const int idx = start / a.P + j, page0 = idx * a.P;        // which page of the row
+  const int idx = page_of(a, start) + j, page0 = idx * a.P;        // which page of the row
   const int lo = max(start, page0), n = min(start + len - page0, a.P) + page0 - lo;
   out.page = a.table[(long)b * a.max_pages + idx];
   out.first = lo - page0;
@@ -982,10 +1002,10 @@ AX_API int ax_kv_write_int8(int dt, const void* k, long k_ts, long k_hs, const v
   const int per_row = T == B ? 1 : (int)((T / B + 2L * P - 2) / P);
   const long pieces = cu == nullptr ? (long)B * per_row : (T + B * (2L * P - 2)) / P + 1;
   if (pieces > 0x7fffffffL) return -3;
-  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, per_row, (65536 + D / 8 - 1) / (D / 8), status};
+  WriteArgs a{k, v, kc, vc, ka, va, table, starts, cu, k_ts, k_hs, v_ts, v_hs, T, B, Hkv, D, P, max_pages, num_pages, per_row, T / B, (P & (P - 1)) == 0 ? __builtin_ctz((unsigned)P) : -1, (65536 + D / 8 - 1) / (D / 8), status};
   const dim3 grid((unsigned)pieces, Hkv);
   // Larger blocks shorten the latency of a big page where few blocks leave room (200 tokens, pages of 64 x 128: 6.2 us
-  // against 8.4); full devices prefer the small ones (8192 tokens, pages of 16 x 128: 19.5 against 32.1).
+  // against 8.4); full devices prefer the small ones (8192 tokens, pages of 16 x 128: 18.5 against 32.1).
   const bool big = (long)P * D >= 4096 && pieces * Hkv < 8L * axh::sm_count();
   auto go = [&](auto kern, int half) { return axh::launch_chained(kern, grid, dim3(2 * half), 0, 1, stream, a); };
   if (dt == 1) return big ? go(kv_write_int8_kernel<__nv_bfloat16, 128>, 128) : go(kv_write_int8_kernel<__nv_bfloat16, 64>, 64);

@@ -421,3 +421,22 @@ def test_write_of_very_many_sequences(B, kernel_status):
     paged.kv_write_int8(k.cuda(), v.cuda(), *gpu, table.cuda(), st.cuda(), cu.int().cuda())
     for a, b in zip(gpu, cpu):
         assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("lens,starts", [([1], [100]), ([100, 0, 7], [47, 5, 48]), ([3] * 40, [i * 5 for i in range(40)])])
+@pytest.mark.parametrize("cu", [True, False])
+def test_pages_of_no_power_of_two(lens, starts, cu, kernel_status):
+    if not cu and len(set(lens)) > 1:
+        lens = [5] * len(lens)
+    Hkv, P, D = 2, 48, 64
+    table, pages = _table([(s + n + P - 1) // P for s, n in zip(starts, lens)])
+    k, v = torch.randn(sum(lens), Hkv, D).bfloat16(), torch.randn(sum(lens), Hkv, D).bfloat16()
+    off = torch.tensor([0] + lens).cumsum(0).int() if cu else None
+    cpu = R.make_cache(pages, Hkv, P, D, "cpu")
+    gpu = [t.cuda() for t in cpu]
+    st = torch.tensor(starts, dtype=torch.int32)
+    paged.kv_write_int8(k, v, *cpu, table, st, off)
+    paged.kv_write_int8(k.cuda(), v.cuda(), *gpu, table.cuda(), st.cuda(), off.cuda() if cu else None)
+    for a, b in zip(gpu, cpu):
+        assert torch.equal(a.cpu(), b)
+    _attend(len(lens), Hkv, 4, D, P, [s + n for s, n in zip(starts, lens)], seed=7)
