@@ -163,8 +163,8 @@ def _gemm_rows(t: torch.Tensor) -> torch.Tensor:
 def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``y = (q * scale) (weight * weight_scale)^T + bias``: ``q`` int8 ``[..., K]`` with ``scale`` ``[...]``,
-    ``weight`` int8 ``[N, K]`` with ``weight_scale`` ``[N]``.  The integer sum is exact; the result is
-    rounded once, to ``out_dtype`` (bf16 or fp32).  K is at most 131071.  Operands whose rows do not start
+    ``weight`` int8 ``[N, K]`` with ``weight_scale`` ``[N]``.  The integer sum is exact, the scales
+    and the bias are applied in fp32, and the result is rounded to ``out_dtype`` (bf16 or fp32).  K is at most 131071.  Operands whose rows do not start
     on 16-byte boundaries are copied first; ``quantize_int8`` and the fused producers lay them out so."""
     if q.dtype is not _I8 or weight.dtype is not _I8:
         raise TypeError("q and weight must be int8")
