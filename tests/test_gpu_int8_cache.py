@@ -440,3 +440,44 @@ def test_pages_of_no_power_of_two(lens, starts, cu, kernel_status):
     for a, b in zip(gpu, cpu):
         assert torch.equal(a.cpu(), b)
     _attend(len(lens), Hkv, 4, D, P, [s + n for s, n in zip(starts, lens)], seed=7)
+
+
+@pytest.mark.parametrize("spare", [0, 9000])
+def test_cache_of_more_than_2_to_the_31_bytes(spare, kernel_status):
+    """Pages at both ends of caches of 2.4 GB each, against the same pages in a small cache."""
+    Hkv, G, P, D, pages = 8, 4, 16, 128, 150_000
+    kc = torch.empty(pages, Hkv, P, D, dtype=torch.int8, device="cuda")
+    vc = torch.empty(pages, Hkv, 1, D, 16, dtype=torch.int8, device="cuda")
+    ka, va = torch.zeros(pages, Hkv, device="cuda"), torch.zeros(pages, Hkv, device="cuda")
+    far = [pages - 1, 0, pages - 2, 131072, 131071, 1, 140_000, 149_000]
+    k, v = torch.randn(2 * 60, Hkv, D, device="cuda").bfloat16(), torch.randn(2 * 60, Hkv, D, device="cuda").bfloat16()
+    q = torch.randn(2, Hkv * G, D, device="cuda").bfloat16()
+    st, cl = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.full((2,), 60, dtype=torch.int32, device="cuda")
+    got = []
+    for caches, ids in (((kc, vc, ka, va), far), (R.make_cache(8, Hkv, P, D, "cuda"), list(range(8)))):
+        table = torch.zeros(2, 4 + spare, dtype=torch.int32)
+        table[:, :4] = torch.tensor(ids).view(2, 4)
+        paged.kv_write_int8(k, v, *caches, table.cuda(), st)
+        got.append((paged.decode_attention_int8(q, *caches, table.cuda(), cl), caches, ids))
+    (a, big, ids), (b, small, _) = got
+    assert torch.equal(a, b)
+    for x, y in zip(big, small):
+        assert torch.equal(x[ids][[0, 1, 2, 4, 5, 6]], y[[0, 1, 2, 4, 5, 6]])
+    assert big[2].count_nonzero() == 8 * Hkv                        # and no other page's magnitude
+
+
+def test_gradients_and_copies_of_unaligned_rows(kernel_status):
+    """Rows off the 16-byte grid and reversed heads are copied; what requires a gradient is refused."""
+    Hkv, P, D = 2, 16, 64
+    c, ref = R.make_cache(2, Hkv, P, D, "cuda", zero=True), R.make_cache(2, Hkv, P, D, "cuda", zero=True)
+    wide = torch.randn(5, Hkv, D + 3, device="cuda").bfloat16()
+    table, st = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda")
+    k, v = wide[..., 3:], wide[..., 1:D + 1].flip(1).transpose(0, 1).contiguous().transpose(0, 1)
+    paged.kv_write_int8(k, v, *c, table, st)
+    paged.kv_write_int8(k.contiguous(), v.contiguous(), *ref, table, st)
+    for a, b in zip(c, ref):
+        assert torch.equal(a, b)
+    with pytest.raises(RuntimeError):
+        paged.kv_write_int8(k.detach().requires_grad_(), v, *c, table, st)
+    with pytest.raises(RuntimeError):
+        paged.decode_attention_int8(torch.randn(1, 2, D, device="cuda").bfloat16().requires_grad_(), *c, table, st + 5)

@@ -188,3 +188,24 @@ def test_more_rows_than_the_kernels_take_are_refused():
     one = torch.ones(1, device="cuda")
     with pytest.raises(ValueError):
         I.int8_linear(q, one.expand(I.MAX_ROWS + 1), q[:1], one)
+
+
+def test_more_than_2_to_the_31_elements(kernel_status):
+    """Rows and products whose offsets pass 32 bits, against the same rows by themselves."""
+    M, K, Nn = 530_000, 4096, 4104
+    x = torch.empty(M, K, dtype=torch.bfloat16, device="cuda").normal_()
+    w = torch.ones(K, device="cuda").bfloat16()
+    last = slice(M - 300, M)
+    q, s = I.quantize_int8(x)
+    q1, s1 = I.quantize_int8(x[last].clone())
+    assert torch.equal(q[last], q1) and torch.equal(s[last], s1)
+    n = I.rms_norm_int8(x, w, residual=x)
+    n1 = I.rms_norm_int8(x[last].clone(), w, residual=x[last].clone())
+    assert all(torch.equal(a[last], b) for a, b in zip(n, n1))
+    del n, n1
+    g, g1 = I.swiglu_int8(x), I.swiglu_int8(x[last].clone())
+    assert torch.equal(g[0][last], g1[0])
+    del g, g1, x
+    W = I.Int8Weight.from_dense(torch.randn(Nn, K, device="cuda"))
+    y = I.int8_linear(q, s, W.q, W.scale)
+    assert y.numel() > 2 ** 31 and torch.equal(y[last], I.int8_linear(q1, s1, W.q, W.scale))
