@@ -43,7 +43,7 @@ class _CountingLib:
 
     _NO_LAUNCH = {"ax_version", "ax_sm_count", "ax_norm_bwd_groups", "ax_multi_tensor_limits", "ax_gemm_comm_set_trace",
                   "ax_flash_fwd_set_trace", "ax_gemm_comm_signal_slots", "ax_norm_bwd_noalloc_limits", "ax_gemm_set_pair_mode", "ax_flash_fwd_set_one_tile", "ax_bounds_enabled", "ax_bounds_read", "ax_gemm_pair_capacity",
-                  "ax_decode_int8_workspace"}
+                  "ax_decode_int8_workspace", "ax_int8_gemm_tile"}
 
     def __init__(self, lib):
         self._lib = lib
@@ -69,6 +69,7 @@ class _CountingLib:
 _SIGNATURES = {
     "ax_int8_rows": "iiipl" "pl" "pf" "pl" "pl" "piip",
     "ax_int8_gemm": "plp" "plp" "ppl" "iiiipp",
+    "ax_int8_gemm_tile": "iiiiip",
     "ax_kv_write_int8": "i" "pll" "pll" "pppp" "ppp" "iiiiiii" "pp",
     "ax_decode_int8": "ppp" "pppp" "p" "iiiiiii" "f" "ppp",
     "ax_decode_int8_workspace": "iiiiii",
@@ -79,7 +80,7 @@ def _declare(lib) -> None:
     kinds = {"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float}
     for name, sig in _SIGNATURES.items():
         getattr(lib, name).argtypes = [kinds[c] for c in sig]
-    lib.ax_decode_int8_workspace.restype = c_int64
+    lib.ax_decode_int8_workspace.restype = lib.ax_int8_gemm_tile.restype = c_int64
 
 
 def bounds_build() -> bool:

@@ -242,6 +242,21 @@ struct PairCfg {
   static constexpr int kSmem = 1024 + kStages * kStage + kEpiWarps * 2 * kStageBuf + 256;
 };
 
+// Tile t of `num_m` x `num_n`: groups of row blocks sweep the columns, so that pairs at work together share tiles in
+// L2.  `group` is at most num_m, so a group's tiles are at most all tiles, which the launch keeps below 2^31.
+__host__ __device__ __forceinline__ void pair_tile(int t, int num_m, int num_n, int group, int& mb, int& nb) {
+  const int per = group * num_n, g = t / per, first = g * group, size = group < num_m - first ? group : num_m - first, r = t - g * per;
+  mb = first + r % size;
+  nb = r / size;
+}
+// Row blocks that sweep together: as many as fill a quarter of L2 with 256 K bytes each, so that they stay there while the
+// weight passes once for all of them.  Back to back under the power cap, 8192 x 28672 x 4096 takes 770 / 740 /
+// 718 / 707 us with 4 / 8 / 16 / 32 together (33 MB), 8192 x 4096 x 14336 365 / 361 / 368 / 394 us (118 MB).
+int pair_group(int M, int K) {
+  const long num_m = ((long)M + 2 * kRowsA - 1) / (2 * kRowsA), fit = (34L << 20) / (256L * K), group = fit < 4 ? 4 : (fit < 1024 ? fit : 1024);
+  return (int)(group < num_m ? group : num_m);
+}
+
 template <int BN, typename OutT>
 __global__ void __launch_bounds__(kThreads, 1)
 int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_w,
@@ -281,20 +296,13 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
   chain_ready();
   chain_wait();
 
-  // groups of row blocks sweep the columns, so that pairs at work together share tiles in L2
-  auto tile_at = [&](int t, int& mb, int& nb) {
-    const int per = p.group * num_n, g = t / per, first = g * p.group, size = min(p.group, num_m - first), r = t - g * per;
-    mb = first + r % size;
-    nb = r / size;
-  };
-
   if (warp == 0) {
     if (lane == 0) {
       int s = 0;
       uint32_t ph = 0;
       for (int t = pair_id; t < num_tiles; t += num_pairs) {
         int mb, nb;
-        tile_at(t, mb, nb);
+        pair_tile(t, num_m, num_n, p.group, mb, nb);
         const int m0 = mb * PM + (int)crank * kRowsA, n0 = nb * BN + (int)crank * HB;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!mbar_wait(&empty[s], ph ^ 1, dead, p.status, 1110)) break;
@@ -348,7 +356,7 @@ int8_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constan
     int buf = 0, it = 0;
     for (int t = pair_id; t < num_tiles; t += num_pairs, ++it) {
       int mb, nb;
-      tile_at(t, mb, nb);
+      pair_tile(t, num_m, num_n, p.group, mb, nb);
       const int m_warp = mb * PM + (int)crank * kRowsA + q * 32, n0 = nb * BN;
       const int acc = it & 1;
       const int m = m_warp + lane;
@@ -519,6 +527,7 @@ int launch_pair(const void* q, long ldq, const void* w, long ldw, const GemmArgs
     if (rc) return 3000 + rc;
   }
   const long tiles = (long)((p.M + 2 * kRowsA - 1) / (2 * kRowsA)) * ((p.N + BN - 1) / BN);
+  if (tiles > 0x7f000000L) return -4;                          // (an output of 2^46 values)
   const int pairs = tiles < max_pairs[dev] ? (int)tiles : max_pairs[dev];
   return axh::launch_chained(kern, dim3(2 * pairs), dim3(kThreads), C::kSmem, 2, stream, mx, mw, mo, p);
 }
@@ -590,12 +599,18 @@ AX_API int ax_int8_gemm(const void* q, long ldq, const float* sx, const void* w,
   if (M <= 0 || N <= 0) return 0;
   if (K <= 0 || K > 131071) return -1;
   if ((ldq % 16) || (ldw % 16) || (((uintptr_t)q | (uintptr_t)w) & 15)) return -2;
-  // Row blocks whose 256 K bytes each fill a quarter of L2 sweep the columns together: they stay there while the
-  // weight passes once for all of them.  Back to back under the power cap, 8192 x 28672 x 4096 takes 770 / 740 /
-  // 718 / 707 us with 4 / 8 / 16 / 32 together (33 MB), 8192 x 4096 x 14336 365 / 361 / 368 / 394 us (118 MB).
-  const long group = (34L << 20) / (256L * K);
-  GemmArgs p{M, N, K, sx, sw, bias, out, ldo, 0, (int)(group < 4 ? 4 : (group < 1024 ? group : 1024)), status};
+  GemmArgs p{M, N, K, sx, sw, bias, out, ldo, 0, pair_group(M, K), status};
   const int size = out_bf16 ? 2 : 4;
   p.tma_out = (ldo * size) % 16 == 0 && ((uintptr_t)out & 15) == 0;
   return out_bf16 ? dispatch<__nv_bfloat16>(q, ldq, w, ldw, p, stream) : dispatch<float>(q, ldq, w, ldw, p, stream);
+}
+
+// Where the many-row kernel puts its tile `t` of `bn` channels for a product of M x N x K: out = {row block, column block}.
+// Returns the number of tiles.  (Host arithmetic alone: what the kernel walks, for its tests.)
+AX_API long ax_int8_gemm_tile(int M, int N, int K, int bn, int t, int* out) {
+  if (M <= 0 || N <= 0 || K <= 0 || bn <= 0) return 0;
+  const int num_m = (M + 2 * kRowsA - 1) / (2 * kRowsA), num_n = (N + bn - 1) / bn;
+  const long tiles = (long)num_m * num_n;
+  if (t >= 0 && t < tiles && tiles <= 0x7f000000L) pair_tile(t, num_m, num_n, pair_group(M, K), out[0], out[1]);
+  return tiles;
 }
