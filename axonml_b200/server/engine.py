@@ -49,6 +49,7 @@ class LLMEngine:
         # CUDA-graph decode: one captured graph per batch size, fed through static input buffers
         self.use_graphs = model.device.type == "cuda" and os.environ.get("AXONML_DECODE_GRAPHS", "1") != "0"
         self._graphs: dict = {}
+        self._graphs_version = getattr(model, "weights_version", 0)
         if self.use_graphs:
             dev = model.device
             if model.tp > 1 and os.environ.get("AXONML_TP_COMM", "fused") == "nccl":
@@ -144,6 +145,15 @@ class LLMEngine:
             if len(r.output) >= r.max_new_tokens or t == r.eos_token_id:
                 self._finish(r, now)
 
+    def _live_graphs(self) -> dict:
+        """The captured graphs by batch size, without those that were captured before the model's weights
+        were replaced (``QuantizedLlama.to_int8``): they would go on reading the freed tensors."""
+        version = getattr(self.model, "weights_version", 0)
+        if version != self._graphs_version:
+            self._graphs.clear()
+            self._graphs_version = version
+        return self._graphs
+
     def _decode_step(self, tokens, slots, positions) -> torch.Tensor:
         """Eager decode, or replay of the CUDA graph captured for this batch size (the whole step -
         embedding gather, 32 layers, head, arg-max - is one graph launch, which removes the
@@ -154,7 +164,7 @@ class LLMEngine:
         self._g_tokens[:B].copy_(tokens)
         self._g_slots[:B].copy_(slots)
         self._g_pos[:B].copy_(positions)
-        g = self._graphs.get(B)
+        g = self._live_graphs().get(B)
         if g is None:
             def run():
                 h = self.model.decode(self._g_tokens[:B], self.cache, self._g_slots[:B], self._g_pos[:B])
@@ -182,7 +192,7 @@ class LLMEngine:
         sizes = sorted(set(batch_sizes or [1, 2, 4, 8, 16, 32, self.max_batch]))
         dev = self.model.device
         for B in sizes:
-            if B in self._graphs or B > self.max_batch:
+            if B in self._live_graphs() or B > self.max_batch:
                 continue
             slots = [self.cache.allocate_seq() for _ in range(B)]
             for sl in slots:

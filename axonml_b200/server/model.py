@@ -46,6 +46,7 @@ class QuantizedLlama:
         cos, sin = Mi.rope_tables(cfg.max_position_embeddings, self.hd, cfg.rope_theta, device=self.device)
         self.cos, self.sin = cos, sin
         self._ar = None
+        self.weights_version = 0      # goes up when weight tensors are replaced: captured graphs hold the old ones' addresses
 
     # ------------------------------------------------------------------ construction
     @classmethod
@@ -177,15 +178,18 @@ class QuantizedLlama:
                 q = getattr(L, name)
                 if ok(q):
                     setattr(L, name, tile_weight(q))
+                    self.weights_version += 1
         if ok(self.head):
             self.head = tile_weight(self.head)
+            self.weights_version += 1
         return self
 
     def to_int8(self) -> "QuantizedLlama":
         """Converts the projections to int8 with one scale per output channel (``ops.int8.Int8Weight``).
         Prefill and decode then run them as int8 products of int8 activations with one scale per token:
         twice the bytes of Q4_K to read when decoding a few sequences, twice the tensor rate of the
-        dequantised product in prefill and large batches.  Embedding and head keep their type."""
+        dequantised product in prefill and large batches.  Embedding and head keep their type.  An engine
+        that serves this model captures its decode graphs anew at its next step."""
         from ..ops.quant import untile_weight
         for L in self.layers:
             for name in ("wqkv", "wo", "wgu", "wdown"):
@@ -194,6 +198,7 @@ class QuantizedLlama:
                     if w.layout == "tile128":
                         w = untile_weight(w)
                     setattr(L, name, I8.Int8Weight.from_dense(dequantize_tensor(w)))
+                    self.weights_version += 1
         return self
 
     def int8_weights(self) -> bool:
