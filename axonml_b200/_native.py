@@ -162,6 +162,22 @@ def check(rc: int, what: str) -> None:
 
 
 _STATUS = {}
+_STATUS_LOCK = threading.Lock()
+
+
+def _capturing(dev: torch.device) -> bool:
+    if dev.type != "cuda":
+        return False
+    with torch.cuda.device(dev):
+        return torch.cuda.is_current_stream_capturing()
+
+
+def _new_status_word(dev: torch.device) -> torch.Tensor:
+    """A status word that is zero for every stream (but inside a capture, where its fill is a node of the graph)."""
+    t = torch.zeros(4, dtype=torch.int32, device=dev)
+    if dev.type == "cuda" and not _capturing(dev):
+        torch.cuda.current_stream(dev).synchronize()
+    return t
 
 
 def status_word(device=None) -> torch.Tensor:
@@ -170,7 +186,10 @@ def status_word(device=None) -> torch.Tensor:
     key = (dev.type, dev.index)
     t = _STATUS.get(key)
     if t is None:
-        t = _STATUS.setdefault(key, torch.zeros(4, dtype=torch.int32, device=dev))    # (one word, also for threads in a race)
+        with _STATUS_LOCK:                                # other host threads see no word, or one that is ready for their streams
+            t = _STATUS.get(key)
+            if t is None:
+                t = _STATUS[key] = _new_status_word(dev)
     return t
 
 
@@ -212,11 +231,9 @@ def status_ptr(index: int) -> int:
     p = _STATUS_PTR.get(index)
     if p is None:
         dev = torch.device("cuda", index)
-        if ("cuda", index) not in _STATUS and torch.cuda.is_current_stream_capturing():
+        if ("cuda", index) not in _STATUS and _capturing(dev):
             raise NativeError("call the operator once before capturing it: its status word does not exist yet")
         p = _STATUS_PTR[index] = status_word(dev).data_ptr()
-        if not torch.cuda.is_current_stream_capturing():
-            torch.cuda.current_stream(dev).synchronize()     # other streams use the word from now on
     return p
 
 
