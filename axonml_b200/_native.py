@@ -76,11 +76,19 @@ _SIGNATURES = {
 }
 
 
+_LONG_RESULTS = ("ax_decode_int8_workspace", "ax_int8_gemm_tile")
+
+
 def _declare(lib) -> None:
+    """Tells ctypes the types of the entry points that ``lib`` has: a library that was built before some of them
+    existed serves the others."""
     kinds = {"p": c_void_p, "i": c_int, "l": c_int64, "f": c_float}
     for name, sig in _SIGNATURES.items():
-        getattr(lib, name).argtypes = [kinds[c] for c in sig]
-    lib.ax_decode_int8_workspace.restype = lib.ax_int8_gemm_tile.restype = c_int64
+        fn = getattr(lib, name, None)
+        if fn is not None:
+            fn.argtypes = [kinds[c] for c in sig]
+            if name in _LONG_RESULTS:
+                fn.restype = c_int64
 
 
 def bounds_build() -> bool:
@@ -211,7 +219,11 @@ def launch(name: str, index: int, *args) -> None:
     last argument), also when that is not the current device, and raises on a non-zero code."""
     fn = _ENTRIES.get(name)
     if fn is None:
-        fn = _ENTRIES[name] = getattr(cuda()._lib, name)
+        fn = getattr(cuda()._lib, name, None)
+        if fn is None:
+            raise NativeError(f"the kernel library has no {name}: it was built before this entry point existed "
+                              "(rebuild it: python -m axonml_b200._build)")
+        _ENTRIES[name] = fn
     _CUDA.launches += 1
     if index == _current_device():
         rc = fn(*args, _current_stream(index))
