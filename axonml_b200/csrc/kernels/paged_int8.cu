@@ -294,11 +294,13 @@ __global__ void __launch_bounds__(2 * kHalf, 512 / kHalf) kv_write_int8_kernel(c
 // with up to eight query heads on the other:
 //   S^T[16 tokens x heads] = K Q^T,      O^T[16 dims x heads] += V^T P^T for each 16 dims
 // int8 becomes fp16 exactly (byte | 0x6400 is 1024 + byte).  Q is scaled by a power of two to lie near one,
-// where fp16 holds every bf16 significand.  P, rounded to fp16 (2^-11, below bf16's own rounding of the
-// result), carries the page's V magnitude relative to the largest one met so far, so that O stays in the
-// accumulators; a page below 1/8 of that is summed apart and added in fp32.
-// The running maximum only moves when a score exceeds it by 2^8 (a vote of the warp finds out): weights up to 256
-// are as exact in fp16 and fp32 as weights up to one, and the usual tile needs no exchange and no rescaling.
+// where fp16 holds every bf16 significand.  P carries the page's V magnitude relative to the largest one met so
+// far, so that O stays in the accumulators; a page below 1/8 of that is summed apart and added in fp32.
+// Weights are counted in 2^-7 of the running maximum's, which only moves when a score exceeds it by 2^8 (a vote of the warp
+// finds out), so that the usual tile needs no exchange and no rescaling: P lies in 0 .. 2^15 and fills fp16's range from
+// above.  Rounding it costs 2^-11 of a weight (below bf16's own rounding of the result) down to 2^-21 of the
+// largest one, and below that 2^-32 of the largest: a long flat tail behind one strong token is still summed, where
+// weights counted from one would vanish at 2^-25.
 //
 // A worker writes a head's result itself when all its tokens were in the worker's share, and otherwise a
 // partial (O, maximum, sum) that a second kernel merges.  Where contexts are short or heads few, the second
@@ -383,8 +385,9 @@ struct AttnCfg {
   static constexpr int kRing = kWarps * kStages * kStage;
   static constexpr int kBlocks = D == 256 ? 2 : 4;               // blocks per SM that registers and shared memory allow
 };
-constexpr float kSlack = 8.f;                                    // log2 of the largest weight
-constexpr float kNone = -3.402823466e38f;                        // running maximum before the first score (-FLT_MAX: not above a finite one)
+constexpr float kUnit = 7.f;                                     // log2 of the weight of a score at the running maximum
+constexpr float kMost = 15.f;                                    // log2 of the largest weight
+constexpr float kNone = -3.402823466e38f;                        // reference before the first score (-FLT_MAX: not above a finite one)
 constexpr float kFaint = 1.f / 8.f;
 
 // NB: blocks of eight query heads.
@@ -514,7 +517,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
   int ctx = 0, s = 0;
   uint32_t ph = 0;
   uint32_t qb[NB][NJ * 4][2];                                    // Q^T: head g of each block, four dims a step
-  // of heads 2 i4 and 2 i4 + 1: scale, running maximum, this lane's share of the sum
+  // of heads 2 i4 and 2 i4 + 1: scale, reference (log2 of the running maximum's weight less kUnit), this lane's share of the sum
   float qs[NB][2], m[NB][2], l[NB][2], o[NB][MT][4];
   float vref = 0.f, vinv = 1.f;                                  // V magnitude (/ 127) that O is counted in, and 1 / it
 #pragma unroll 1
@@ -631,7 +634,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
-        for (int c = 0; c < 2; ++c) move |= fmaxf(sc[nb][c], sc[nb][2 + c]) > m[nb][c] + kSlack;
+        for (int c = 0; c < 2; ++c) move |= fmaxf(sc[nb][c], sc[nb][2 + c]) > m[nb][c] + kMost;
       if (__any_sync(0xffffffffu, move)) {
         const float vnew = fmaxf(vref, va), down = vnew > 0.f ? __fdiv_rn(vref, vnew) : 1.f;
 #pragma unroll
@@ -642,7 +645,7 @@ __global__ void __launch_bounds__(kWarps * 32, NB == 1 ? AttnCfg<D>::kBlocks : 2
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
             mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
-            const float mn = mx > m[nb][c] + kSlack ? mx : m[nb][c];
+            const float mn = mx > m[nb][c] + kMost ? mx - kUnit : m[nb][c];
             const float alpha = exp2f(m[nb][c] - mn);
             m[nb][c] = mn;
             l[nb][c] *= alpha;
