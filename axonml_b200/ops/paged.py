@@ -66,6 +66,7 @@ def decode_attention(q, k_cache, v_cache, block_table, ctx_lens, page_size: int,
 
 # ------------------------------------------------------------------------------ cache in 8 bits
 _I8, _I32, _F32 = torch.int8, torch.int32, torch.float32
+_MAX_TILES = 0x7f000000      # 16-token tiles, over sequences and KV heads, that one launch of the attention can number
 
 
 def _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table):
@@ -187,7 +188,8 @@ def _kv_write_int8_cpu(k, v, k_cache, v_cache, k_amax, v_amax, block_table, star
 def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_lens, scale: float | None = None):
     """Attention of one query token per sequence over an int8 cache (laid out as ``kv_write_int8``
     says): ``q`` bf16 ``[B, Hq, D]`` -> ``[B, Hq, D]``, each sequence over its first ``ctx_lens[b]`` tokens; an
-    empty context gives zeros.  On a GPU D is 64, 128 or 256; any number of query heads per KV head.  A
+    empty context gives zeros.  On a GPU D is 64, 128 or 256; any number of query heads per KV head; a
+    sequence's table has room for at most 2^31 / KV heads tiles of 16 tokens (with more than 16 query heads per KV head, as often less).  A
     page number outside the cache and a context longer than the table are reported by
     ``_native.check_status()`` and not read."""
     pages, Hkv, P, D, index = _check_int8_cache(k_cache, v_cache, k_amax, v_amax, block_table)
@@ -212,8 +214,8 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
         q = q.clone(memory_format=torch.contiguous_format)
     out = torch.empty_like(q)
     table = block_table if block_table.is_contiguous() else block_table.contiguous()
-    each = B if B <= 1024 else -(-B // -(-B // 1024))  # the kernel keeps a running count per sequence in shared memory
-    for b0 in range(0, B, each or 1):
+    each = _int8_sequences(B, Hq // Hkv, Hkv, width, P)
+    for b0 in range(0, B, each):
         n = min(each, B - b0)
         size = _int8_workspace(index, n, Hq, Hkv, D, width, P)
         ws = k_amax.new_empty(size) if size else None
@@ -221,6 +223,17 @@ def decode_attention_int8(q, k_cache, v_cache, k_amax, v_amax, block_table, ctx_
                  v_amax.data_ptr(), table.data_ptr() + b0 * width * 4, ctx_lens.data_ptr() + b0 * 4, out.data_ptr() + b0 * Hq * D * 2, n, Hq, Hkv,
                  D, P, width, pages, scale, ws.data_ptr() if size else 0, N.status_ptr(index))
     return out
+
+
+def _int8_sequences(B: int, G: int, Hkv: int, width: int, P: int) -> int:
+    """Sequences of one launch, in shares as even as they can be: the kernel keeps a running count for each of at most 1024
+    in shared memory, and numbers the 16-token tiles that a launch's tables have room for in 31 bits."""
+    tiles = Hkv * (1 if G <= 8 else -(-G // 16)) * width * (P // 16)
+    most = min(1024, _MAX_TILES // max(tiles, 1))
+    if most == 0:
+        raise ValueError(f"a table of {width} pages of {P} tokens with {Hkv} KV heads and {G} query heads each is more than the kernel takes "
+                         f"({_MAX_TILES} tiles of 16 tokens and up to 16 query heads)")
+    return -(-B // -(-B // most)) if B else 1
 
 
 @functools.lru_cache(maxsize=4096)
