@@ -28,6 +28,13 @@ __device__ __forceinline__ void from_f(float v, __nv_bfloat16* p) { *p = __float
 __device__ __forceinline__ float round_to(float v, const float*) { return v; }
 __device__ __forceinline__ float round_to(float v, const __nv_bfloat16*) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
+// x + r as the stream's type rounds it.  The files are compiled with subnormal results flushed to zero; the stream keeps its own.
+__device__ __forceinline__ float add_stream(float x, float r) {
+  float h;
+  asm("add.rn.f32 %0, %1, %2;" : "=f"(h) : "f"(x), "f"(r));
+  return h;
+}
+
 struct RowArgs {
   const void* x;      // [rows, D], or [rows, 2 D] gate | up
   const void* res;    // [rows, D] or null
@@ -113,7 +120,7 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSw
         if (MODE == kNorm) {
           if (RES) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) t[i][j] += u[j];
+            for (int j = 0; j < 8; ++j) t[i][j] = add_stream(t[i][j], u[j]);
             first[i].set(t[i]);                              // the stream's own rounding
             first[i].store((T*)a.h + row * a.hs + c);
           }
@@ -217,7 +224,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) int8_rows_any_kernel(const 
       if (MODE == kSwiglu) v[j] = siluf_(v[j]) * u[j];
       if (MODE == kNorm) {
         if (RES) {
-          v[j] = round_to(v[j] + u[j], (const T*)nullptr);
+          v[j] = round_to(add_stream(v[j], u[j]), (const T*)nullptr);
           if (out && j * n < left) from_f(v[j], (T*)a.h + row * a.hs + c0 + tid + j * n);
         }
         sum += v[j] * v[j];
