@@ -45,6 +45,7 @@ struct RowArgs {
   long xs, rs, hs, qs;
   int D;
   float eps;
+  float least;        // sums of squares below this may lack some that vanished: 2^-100 D without an eps that hides it, else 0
 };
 
 // Sum (where SUM) and largest bits over the block; every thread gets both.  `turn` alternates between two sets of
@@ -67,6 +68,48 @@ template <int MODE>
 __device__ __forceinline__ void write_scale(const RowArgs& a, long row, float sum, uint32_t top) {
   const float rstd = MODE == kNorm ? __frsqrt_rn(__fdiv_rn(sum, (float)a.D) + a.eps) : 1.f;
   a.scale[row] = __fdiv_rn(__fmul_rn(top < kTinyBits ? 0.f : __uint_as_float(top), rstd), 127.f);
+}
+
+// A norm whose sums left fp32's range: squares that overflow (values above about 1e19), t = h w that does, or squares that
+// vanish beside an eps that is nothing either.  (A row with a value that is not finite comes here too, and keeps its scale that is not.)
+__device__ __forceinline__ bool norm_out_of_range(const RowArgs& a, float sum, uint32_t top) {
+  return !(sum >= a.least && sum <= 3.402823466e38f) || top >= 0x7f800000u;
+}
+// Such a row again, when the block has nothing else left: its values scaled by the power of two that brings the largest |h| near
+// one and cancels, y = t f / sqrt(mean (h f)^2 + eps f^2).  Three walks; h has been stored.
+template <bool RES, typename T, typename WT>
+__device__ __forceinline__ void norm_scaled_row(const RowArgs& a, long row) {
+  const int tid = threadIdx.x, n = blockDim.x;
+  const T* x = (const T*)a.x + row * a.xs;
+  const T* r = RES ? (const T*)a.res + row * a.rs : x;
+  const WT* w = (const WT*)a.w;
+  auto value = [&](int c) {
+    const float v = to_f(x[c]);
+    return RES ? round_to(add_stream(v, to_f(r[c])), (const T*)nullptr) : v;
+  };
+  float most = 0.f, sum = 0.f;
+#pragma unroll 1
+  for (int c = tid; c < a.D; c += n) most = amax_nan(most, value(c));
+  __syncthreads();                                             // what the first pass wrote lies before what follows
+  uint32_t top = abs_bits(most);
+  block_stats<false>(sum, top, 0);
+  const int up = top >= 0x7f800000u ? 0 : min(max(127 - (int)(top >> 23), -126), 100);
+  const float f = __uint_as_float((uint32_t)(127 + up) << 23);
+  sum = most = 0.f;
+#pragma unroll 1
+  for (int c = tid; c < a.D; c += n) {
+    const float v = value(c) * f;
+    sum += v * v;
+    most = amax_nan(most, __fmul_rn(v, to_f(w[c])));
+  }
+  top = abs_bits(most);
+  block_stats<true>(sum, top, 0);
+  const Int8Grid grid = int8_grid(top);
+  RowArgs b = a;
+  b.eps = a.eps * f * f;
+  if (tid == 0) write_scale<kNorm>(b, row, sum, top);
+#pragma unroll 1
+  for (int c = tid; c < a.D; c += n) a.q[row * a.qs + c] = (int8_t)int8_bits(__fmul_rn(value(c) * f, to_f(w[c])), grid);
 }
 
 // Rows and D allow 16-byte accesses, and VPT groups of eight values a thread cover a row.
@@ -94,6 +137,7 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSw
   };
   chain_ready();
   chain_wait();
+  bool again = false;
   long row = blockIdx.x;
   if (kAhead) request(row);
   if (MODE == kNorm) {
@@ -143,13 +187,29 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSw
     uint32_t top = abs_bits(most);
     block_stats<MODE == kNorm>(sum, top, turn);
     const Int8Grid grid = int8_grid(top);
-    if (tid == 0) write_scale<MODE>(a, row, sum, top);
+    const bool out = MODE == kNorm && norm_out_of_range(a, sum, top);
+    again |= out;                                            // (uniform)
+    if (tid == 0) {
+      if (out) a.scale[row] = __uint_as_float(0x7fffffffu);  // found below: no other row's scale is a NaN
+      else write_scale<MODE>(a, row, sum, top);
+    }
     int8_t* q = a.q + row * a.qs;
 #pragma unroll
     for (int i = 0; i < VPT; ++i) {
       const int c = (i * n + tid) * 8;
       const uint2 b = int8_steps(t[i], grid);
       if (c < a.D) *reinterpret_cast<uint2*>(q + c) = b;
+    }
+  }
+  if constexpr (MODE == kNorm) {
+    if (again) {
+      __syncthreads();
+#pragma unroll 1
+      for (row = blockIdx.x; row < rows; row += gridDim.x) {
+        const bool marked = abs_bits(a.scale[row]) > 0x7f800000u;
+        __syncthreads();                                     // all have read the mark, and the row before is done
+        if (marked) norm_scaled_row<RES, T, WT>(a, row);
+      }
     }
   }
 }
@@ -243,6 +303,7 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) int8_rows_any_kernel(const 
   uint32_t top = abs_bits(most);
   block_stats<MODE == kNorm>(sum, top, 0);
   const Int8Grid grid = int8_grid(top);
+  const bool again = MODE == kNorm && norm_out_of_range(a, sum, top);
   if (tid == 0) write_scale<MODE>(a, row, sum, top);
   int8_t* q = a.q + row * a.qs + tid;
 #pragma unroll
@@ -254,6 +315,9 @@ __global__ void __launch_bounds__(KEEP ? 512 : 1024) int8_rows_any_kernel(const 
 #pragma unroll
     for (int j = 0; j < 8; ++j)
       if (j * n < left) q[8 * n * k + j * n] = (int8_t)((j < 4 ? b.x : b.y) >> (8 * (j % 4)));
+  }
+  if constexpr (MODE == kNorm) {
+    if (again) norm_scaled_row<RES, T, WT>(a, row);
   }
 }
 
@@ -338,7 +402,8 @@ AX_API int ax_int8_rows(int mode, int dt, int wdt, const void* x, long xs, const
                         void* h, long hs, int8_t* q, long qs, float* scale, int rows, int D, cudaStream_t stream) {
   if (rows <= 0 || D <= 0) return 0;
   if (mode < 0 || mode > 2 || (mode == kNorm && w == nullptr) || ((res == nullptr) != (h == nullptr))) return -1;
-  RowArgs a{x, res, w, h, q, scale, xs, rs, hs, qs, D, eps};
+  constexpr float kLeast = 7.888609052e-31f;                   // 2^-100: a square that vanishes (below 2^-126) is 2^-26 of that
+  RowArgs a{x, res, w, h, q, scale, xs, rs, hs, qs, D, eps, eps < kLeast ? kLeast * (float)D : 0.f};
   using bf = __nv_bfloat16;
   if (mode == kNorm) {
     if (dt == 1 && wdt == 1) return launch_norm<bf, bf>(a, rows, stream);

@@ -49,6 +49,16 @@ def _ref_rows(t: torch.Tensor, norm=None):
     return _steps(t, amax), scale.squeeze(-1).float()
 
 
+def _ref_norm_rows(h: torch.Tensor, w: torch.Tensor, eps: float):
+    mean = h.square().mean(-1, keepdim=True) + eps
+    top = h.abs().amax(-1, keepdim=True)
+    # sums outside fp32's range: values scaled by a power of two, which cancels
+    out = ~((mean >= 2.0 ** -100) & mean.isfinite() & (h * w).isfinite().all(-1, keepdim=True)) & top.isfinite()
+    f = torch.where(out, torch.ldexp(torch.ones_like(top), (1 - top.frexp().exponent).clamp(-126, 100)), torch.ones_like(top))
+    h = h * f
+    return _ref_rows(h * w, torch.rsqrt(h.square().mean(-1, keepdim=True) + eps * f * f))
+
+
 _I8, _F32 = torch.int8, torch.float32
 _KINDS = {torch.bfloat16: 1, torch.float32: 0}
 
@@ -119,13 +129,16 @@ def quantize_int8(x: torch.Tensor):
 
 def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: torch.Tensor | None = None):
     """RMSNorm over the last dim, to int8 rows: ``(q, scale)``.  With ``residual`` the norm is of
-    ``h = x + residual`` (rounded to ``x``'s type) and the result is ``(q, scale, h)``."""
+    ``h = x + residual`` (rounded to ``x``'s type) and the result is ``(q, scale, h)``.  Rows whose squares leave
+    fp32's range (values above about 1e19; tiny ones with an ``eps`` of nothing) are scaled by a power of two first."""
     _check_rows(x)
     D, dev = x.shape[-1], x.get_device()                   # (-1: not on a GPU)
     if weight.dim() != 1 or weight.shape[0] != D:
         raise ValueError(f"weight {tuple(weight.shape)} does not fit rows of {D}")
     if weight.get_device() != dev:
         raise ValueError(f"weight is on {weight.device}, x on {x.device}")
+    if 0 < abs(eps) < 2.0 ** -126:
+        raise ValueError(f"eps must be 0 or a normal fp32 number, not {eps}")
     if weight.requires_grad:
         _no_gradient()
     if residual is not None:
@@ -137,8 +150,7 @@ def rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resi
         q, scale, h = _launch_rows(1, x, D, residual, weight, eps)
     else:
         h = x if residual is None else x + residual
-        hf = h.float()
-        q, scale = _ref_rows(hf * weight.float(), torch.rsqrt(hf.square().mean(-1, keepdim=True) + eps))
+        q, scale = _ref_norm_rows(h.float(), weight.float(), eps)
     return (q, scale, h) if residual is not None else (q, scale)
 
 
