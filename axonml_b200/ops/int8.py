@@ -166,12 +166,6 @@ def swiglu_int8(gate_up: torch.Tensor):
     return _ref_rows(torch.nn.functional.silu(g) * u)
 
 
-def _gemm_rows(t: torch.Tensor) -> torch.Tensor:
-    if t.stride(1) == 1 and t.stride(0) % 16 == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return _aligned_rows(t.shape[0], t.shape[1], t.device).copy_(t)
-
-
 def int8_linear(q: torch.Tensor, scale: torch.Tensor, weight: torch.Tensor, weight_scale: torch.Tensor, bias: torch.Tensor | None = None,
                 out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``y = (q * scale) (weight * weight_scale)^T + bias``: ``q`` int8 ``[..., K]`` with ``scale`` ``[...]``,
