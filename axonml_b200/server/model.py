@@ -19,6 +19,7 @@ from ..ops import elementwise as E
 from ..ops import int8 as I8
 from ..ops import misc as Mi
 from ..ops import norm as Nm
+from ..ops import paged
 from ..ops.attention import sdpa
 from ..ops.quant import qlinear
 from ..quant.quantize import dequantize_tensor, quantize_tensor
@@ -27,6 +28,19 @@ from ..quant.types import QuantizedTensor, QuantType
 
 class _Layer:
     __slots__ = ("attn_norm", "wqkv", "wo", "ffn_norm", "wgu", "wdown")
+
+
+def _write(cache, layer, k, v, table, starts, seq, positions) -> None:
+    if hasattr(cache, "write"):
+        cache.write(layer, k, v, table, starts, seq, positions)
+    else:
+        paged.kv_write(k, v, cache.k[layer], cache.v[layer], table, seq, positions, cache.page_size)
+
+
+def _attend(cache, layer, q, table, ctx):
+    if hasattr(cache, "attend"):
+        return cache.attend(layer, q, table, ctx)
+    return paged.decode_attention(q, cache.k[layer], cache.v[layer], table, ctx, cache.page_size)
 
 
 class QuantizedLlama:
@@ -284,13 +298,14 @@ class QuantizedLlama:
 
     def prefill(self, ids: torch.Tensor, cache, slots, layer_write=True) -> torch.Tensor:
         """``ids`` [B, S] (equal-length prompts); writes K/V of every token into the pages of
-        ``slots`` and returns the hidden state of the last token of each prompt, [B, H]."""
+        ``slots`` and returns the hidden state of the last token of each prompt, [B, H].  ``cache`` is a
+        ``PagedKVCache`` or holds bf16 pages as one does (``k``, ``v``, ``block_table``, ``page_size``)."""
         B, S = ids.shape
         x = self._embed(ids).view(B * S, -1)
         seq = torch.tensor(slots, dtype=torch.int32, device=self.device).repeat_interleave(S)
         pos = torch.arange(S, dtype=torch.int32, device=self.device).repeat(B)
         table, starts, rows = cache.block_table, None, seq
-        if cache.int8:
+        if getattr(cache, "int8", False):
             table = cache.block_table[torch.tensor(slots, dtype=torch.long, device=self.device)]
             starts = torch.zeros(B, dtype=torch.int32, device=self.device)
         nq, nk = self.hq * self.hd, self.hkv * self.hd
@@ -305,7 +320,7 @@ class QuantizedLlama:
             qkv = qkv.view(B * S, self.hq + 2 * self.hkv, self.hd)
             qkv = Mi.rope_positions(qkv, self.cos, self.sin, pos, rot_heads=self.hq + self.hkv)
             q, k, v = qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv], qkv[:, self.hq + self.hkv:]
-            cache.write(li, k, v, table, starts, rows, pos)
+            _write(cache, li, k, v, table, starts, rows, pos)
             a = sdpa(q.reshape(B, S, self.hq, self.hd), k.reshape(B, S, self.hkv, self.hd),
                      v.reshape(B, S, self.hkv, self.hd), causal=True)
             if int8:
@@ -334,7 +349,8 @@ class QuantizedLlama:
         activations itself and RoPE + KV write are one launch (``ops/decode.py``)."""
         import os
         from ..ops import decode as Dc
-        if os.environ.get("AXONML_DECODE_FUSED", "1") == "0" or self.hd != 128 or not self.layers or cache.int8 or self.int8_weights():
+        if os.environ.get("AXONML_DECODE_FUSED", "1") == "0" or self.hd != 128 or not self.layers or self.int8_weights() \
+                or getattr(cache, "int8", False):
             return False
         from .. import _native as N
         L = self.layers[0]
@@ -389,8 +405,8 @@ class QuantizedLlama:
             qkv = (self._rows_linear(h, L.wqkv) if int8 else qlinear(h, L.wqkv)).view(B, self.hq + 2 * self.hkv, self.hd)
             qkv = Mi.rope_positions(qkv, self.cos, self.sin, positions, rot_heads=self.hq + self.hkv)
             q, k, v = qkv[:, :self.hq], qkv[:, self.hq:self.hq + self.hkv], qkv[:, self.hq + self.hkv:]
-            cache.write(li, k, v, table, positions, seq_local, positions)
-            a = cache.attend(li, q.contiguous(), table, ctx)
+            _write(cache, li, k, v, table, positions, seq_local, positions)
+            a = _attend(cache, li, q.contiguous(), table, ctx)
             nxt = self.layers[li + 1].attn_norm if li + 1 < len(self.layers) else None
             if int8:
                 o = self._all_reduce(L.wo.linear(a.reshape(B, nq)))

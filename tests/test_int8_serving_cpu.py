@@ -1,4 +1,6 @@
 """The serving engine and model around int8 weights and caches, on the CPU path."""
+import types
+
 import torch
 
 from axonml_b200 import llm, server
@@ -22,3 +24,21 @@ def test_graphs_of_replaced_weights_are_dropped():
     eng._graphs[2] = "captured again"
     m.to_int8()                                          # nothing is replaced
     assert eng._live_graphs() == {2: "captured again"}
+
+
+def test_a_plain_holder_of_pages_serves_as_a_cache():
+    """prefill and decode take any object with bf16 pages and a block table, as before there were int8 caches."""
+    m = _model()
+    ids = torch.randint(0, 512, (2, 9), generator=torch.Generator().manual_seed(1))
+    slots = torch.tensor([0, 1], dtype=torch.int32)
+    got = []
+    with torch.no_grad():
+        for plain in (False, True):
+            c = server.PagedKVCache(2, 8, 4, m.hkv, m.hd, 2, 4, "cpu")
+            for s in (c.allocate_seq(), c.allocate_seq()):
+                c.reserve(s, 10)
+            if plain:
+                c = types.SimpleNamespace(k=c.k, v=c.v, block_table=c.block_table, page_size=c.page_size)
+            h = m.prefill(ids, c, [0, 1])
+            got.append((h, m.decode(torch.tensor([5, 6]), c, slots, torch.tensor([9, 9], dtype=torch.int32))))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
