@@ -704,6 +704,8 @@ def cmd_serve(a):
     from ..server.http import AxonmlHTTPServer
     from ..server.inference import InferenceServer
     engine = None
+    if not a.gguf and (a.weights == "int8" or a.kv_cache == "int8"):
+        raise SystemExit("--weights int8 and --kv-cache int8 are for the language model of --gguf")
     if a.gguf:
         from ..server import LLMEngine, QuantizedLlama
         model = QuantizedLlama.from_gguf(a.gguf, device="cuda" if torch.cuda.is_available() else "cpu")

@@ -1,6 +1,7 @@
 """The serving engine and model around int8 weights and caches, on the CPU path."""
 import types
 
+import pytest
 import torch
 
 from axonml_b200 import llm, server
@@ -42,3 +43,12 @@ def test_a_plain_holder_of_pages_serves_as_a_cache():
             h = m.prefill(ids, c, [0, 1])
             got.append((h, m.decode(torch.tensor([5, 6]), c, slots, torch.tensor([9, 9], dtype=torch.int32))))
     assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+@pytest.mark.parametrize("flags", [["--kv-cache", "int8"], ["--weights", "int8"]])
+def test_int8_flags_without_a_language_model_are_refused(flags, monkeypatch):
+    from axonml_b200.cli.main import main
+    from axonml_b200.server import http
+    monkeypatch.setattr(http.AxonmlHTTPServer, "serve_forever", lambda self: None)
+    with pytest.raises(SystemExit, match="gguf"):
+        main(["serve", "--port", "0", *flags])
