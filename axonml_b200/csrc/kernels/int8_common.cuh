@@ -34,22 +34,36 @@ __device__ __forceinline__ float amax_nan(float a, float x) {
 struct Int8Grid {
   float hi, lo;        // n / a as a sum of two floats; 0 for a group whose steps are all 0
 };
-constexpr uint32_t kTinyBits = 7u << 23;   // 2^-120: below it a group counts as zero (127 / a would overflow)
-__device__ __forceinline__ Int8Grid int8_grid(uint32_t top, float n = 127.f) {
-  Int8Grid g{0.f, 0.f};
-  if (top >= kTinyBits && top < 0x7f800000u) {
-    const float a = __uint_as_float(top);
-    g.hi = __fdiv_rn(n, a);
-    g.lo = __fdividef(__fmaf_rn(-g.hi, a, n), a);
-  }
+// 2^-118: below it a group counts as zero.  From there on a / 127 is a normal number, and a value that is not (the files are
+// compiled with those flushed to zero) is less than half a step.
+constexpr uint32_t kTinyBits = 9u << 23;
+__device__ __forceinline__ Int8Grid two_float_quotient(float n, float a) {
+  Int8Grid g;
+  g.hi = __fdiv_rn(n, a);
+  // (the small part of 127 / a is below the normal numbers from a = 2^108 on: kept, to 2^-150, which times a value below 2^128
+  // is far less than the quotient's last bit)
+  asm("div.full.f32 %0, %1, %2;" : "=f"(g.lo) : "f"(__fmaf_rn(-g.hi, a, n)), "f"(a));
   return g;
+}
+__device__ __forceinline__ Int8Grid int8_grid(uint32_t top) {
+  if (top < kTinyBits || top >= 0x7f800000u) return Int8Grid{0.f, 0.f};
+  return two_float_quotient(127.f, __uint_as_float(top));
+}
+// From magnitude `old_bits` to a larger one, both times 2^64 where the quotient's remainder would be below the normal numbers.
+__device__ __forceinline__ Int8Grid int8_ratio(uint32_t old_bits, uint32_t top) {
+  if (top < kTinyBits || top >= 0x7f800000u) return Int8Grid{0.f, 0.f};
+  const float f = top < (87u << 23) ? 18446744073709551616.f : 1.f;      // 2^-40
+  return two_float_quotient(__uint_as_float(old_bits) * f, __uint_as_float(top) * f);
 }
 
 // Adding 1.5 * 2^23 rounds a number below 2^22 to the nearest whole one (ties to even) and leaves that number,
 // in two's complement, in the low bits of the sum: no conversion instruction, which the SM has at a
 // sixteenth of the rate of additions.
 __device__ __forceinline__ uint32_t int8_bits(float t, const Int8Grid& g) {
-  return __float_as_uint(__fadd_rn(__fmaf_rn(t, g.hi, __fmul_rn(t, g.lo)), 12582912.f));
+  float low, q;
+  asm("mul.rn.f32 %0, %1, %2;" : "=f"(low) : "f"(t), "f"(g.lo));
+  asm("fma.rn.f32 %0, %1, %2, %3;" : "=f"(q) : "f"(t), "f"(g.hi), "f"(low));
+  return __float_as_uint(__fadd_rn(q, 12582912.f));
 }
 
 __device__ __forceinline__ uint32_t pack_low_bytes(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {

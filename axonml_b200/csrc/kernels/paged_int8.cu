@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(2 * kHalf, 512 / kHalf) kv_write_int8_kernel(c
   if (top < kTinyBits) top = 0;
   const Int8Grid grid = int8_grid(top);
   const bool again = top > old_bits && pc.first > 0;       // the page's magnitude grows
-  const Int8Grid shrink = int8_grid(again ? top : 0u, __uint_as_float(old_bits));
+  const Int8Grid shrink = int8_ratio(old_bits, again ? top : 0u);
   if (tid == 0) *amax_p = __uint_as_float(top);
 
   if (again) {                                               // what the page held: whole tokens of K, whole 16-slot groups of V

@@ -33,7 +33,7 @@ def _no_gradient() -> None:
         raise RuntimeError("the int8 operators have no gradient: call them under torch.no_grad()")
 
 
-TINY = 2.0 ** -120      # a group whose largest magnitude is below this counts as zero
+TINY = 2.0 ** -118      # a group whose largest magnitude is below this counts as zero (its scale would not be a normal number)
 
 
 def _steps(t: torch.Tensor, amax: torch.Tensor) -> torch.Tensor:
