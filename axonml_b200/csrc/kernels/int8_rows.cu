@@ -112,6 +112,11 @@ __device__ __forceinline__ void norm_scaled_row(const RowArgs& a, long row) {
   for (int c = tid; c < a.D; c += n) a.q[row * a.qs + c] = (int8_t)int8_bits(__fmul_rn(value(c) * f, to_f(w[c])), grid);
 }
 
+// Inlined behind the loop over rows it costs that loop 6 % without a residual (8192 x 4096 bf16: 22.4 us, 21.3 as a call), and as a call
+// 3 % with one (fp32: 83.7 inlined, 86.2).
+template <typename T, typename WT>
+__device__ __noinline__ void norm_scaled_row_call(const RowArgs a, long row) { norm_scaled_row<false, T, WT>(a, row); }
+
 // Rows and D allow 16-byte accesses, and VPT groups of eight values a thread cover a row.
 template <int MODE, bool RES, typename T, typename WT, int VPT>
 __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSwiglu ? 2 : 1) int8_rows_kernel(const RowArgs a, int rows) {
@@ -208,7 +213,9 @@ __global__ void __launch_bounds__(VPT == 4 ? 512 : 1024, VPT == 4 && MODE == kSw
       for (row = blockIdx.x; row < rows; row += gridDim.x) {
         const bool marked = abs_bits(a.scale[row]) > 0x7f800000u;
         __syncthreads();                                     // all have read the mark, and the row before is done
-        if (marked) norm_scaled_row<RES, T, WT>(a, row);
+        if (!marked) continue;
+        if constexpr (RES) norm_scaled_row<true, T, WT>(a, row);
+        else norm_scaled_row_call<T, WT>(a, row);
       }
     }
   }
