@@ -11,7 +11,7 @@
 // next row is requested before that reduction, so that its loads travel while this row is rounded.  Rows too
 // wide for registers are read twice, the second time from L2.  The kernels are bound by the bytes of x, r, h
 // and q, in so far as a row's 15 to 24 instructions a value leave room: norm of 8192 x 4096 bf16 with a
-// residual 37.9 us (6.2 TB/s), SwiGLU of 4096 x 11008 45.2 us (5.0 TB/s: two special-function results and some 20
+// residual 37.4 us (6.3 TB/s), SwiGLU of 4096 x 11008 45.4 us (5.0 TB/s: two special-function results and some 20
 // instructions a value), 1021 x 5125 fp32 rows off the 16-byte grid 11 us.
 #include "int8_common.cuh"
 

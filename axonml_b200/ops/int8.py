@@ -3,7 +3,8 @@ int8 matrix (``csrc/kernels/int8_rows.cu``, ``int8_gemm.cu``).
 
 A value is ``q * scale`` with ``q`` in [-127, 127] and one fp32 scale per row (a token of the
 activations, an output channel of a weight).  The producers round as the real numbers would:
-``q = rint(127 y / max|y|)``, ties to even; a row below ``TINY`` everywhere counts as zero, one with
+``q = rint(127 y / max|y|)``, ties to even (of SwiGLU's ``y`` as fp32 holds it: its exponential is approximate, so a step
+next to a border may be its neighbour); a row below ``TINY`` everywhere counts as zero, one with
 a value that is not finite gets a scale that is not.  For inference; nothing here has a gradient.  CPU tensors
 take the same maths in torch."""
 from __future__ import annotations

@@ -31,7 +31,8 @@ class Request:
 class LLMEngine:
     def __init__(self, model, max_batch: int = 64, max_context: int = 1024, page_size: int = 16,
                  num_pages: int | None = None, kv_dtype: torch.dtype = torch.bfloat16):
-        """``kv_dtype``: bf16, or int8 for a cache of half the size (pages of a multiple of 16 tokens)."""
+        """``kv_dtype``: bf16, or int8 for a cache of half the size (pages of a multiple of 16 tokens; without the fused
+        decode step that block-quantised weights and up to four sequences have with bf16)."""
         if kv_dtype not in (torch.bfloat16, torch.int8):
             raise ValueError(f"kv_dtype must be bf16 or int8, not {kv_dtype}")
         self.model, self.max_batch = model, max_batch

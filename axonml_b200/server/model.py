@@ -201,8 +201,8 @@ class QuantizedLlama:
     def to_int8(self) -> "QuantizedLlama":
         """Converts the projections to int8 with one scale per output channel (``ops.int8.Int8Weight``).
         Prefill and decode then run them as int8 products of int8 activations with one scale per token:
-        twice the bytes of Q4_K to read when decoding a few sequences, twice the tensor rate of the
-        dequantised product in prefill and large batches.  Embedding and head keep their type.  An engine
+        twice the bytes of Q4_K to read, which a single sequence feels (383 tok/s against 411, 8B architecture), no
+        dequantisation, which pays from a few sequences on (four: 1440 against 798), and twice the tensor rate in prefill.  Embedding and head keep their type.  An engine
         that serves this model captures its decode graphs anew at its next step."""
         from ..ops.quant import untile_weight
         for L in self.layers:
