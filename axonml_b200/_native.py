@@ -181,10 +181,14 @@ def _capturing(dev: torch.device) -> bool:
 
 
 def _new_status_word(dev: torch.device) -> torch.Tensor:
-    """A status word that is zero for every stream (but inside a capture, where its fill is a node of the graph)."""
-    t = torch.zeros(4, dtype=torch.int32, device=dev)
-    if dev.type == "cuda" and not _capturing(dev):
-        torch.cuda.current_stream(dev).synchronize()
+    """A status word that is zero for every stream (but inside a capture, where its fill is a node of the graph).  It is
+    filled on a stream of its own, so that the wait for it is not one for the work that is queued already."""
+    if dev.type != "cuda" or _capturing(dev):
+        return torch.zeros(4, dtype=torch.int32, device=dev)
+    side = torch.cuda.Stream(dev)
+    with torch.cuda.stream(side):
+        t = torch.zeros(4, dtype=torch.int32, device=dev)
+    side.synchronize()
     return t
 
 
