@@ -93,7 +93,11 @@ __device__ __forceinline__ void norm_scaled_row(const RowArgs& a, long row) {
   __syncthreads();                                             // what the first pass wrote lies before what follows
   uint32_t top = abs_bits(most);
   block_stats<false>(sum, top, 0);
-  const int up = top >= 0x7f800000u ? 0 : min(max(127 - (int)(top >> 23), -126), 100);
+  if (top >= 0x7f800000u) {                                    // a value that is not finite: so is the scale
+    if (tid == 0) a.scale[row] = __uint_as_float(0x7fffffffu);
+    return;
+  }
+  const int up = min(max(127 - (int)(top >> 23), -126), 100);
   const float f = __uint_as_float((uint32_t)(127 + up) << 23);
   sum = most = 0.f;
 #pragma unroll 1
