@@ -203,7 +203,8 @@ class QuantizedLlama:
         Prefill and decode then run them as int8 products of int8 activations with one scale per token:
         twice the bytes of Q4_K to read, which a single sequence feels (383 tok/s against 411, 8B architecture), no
         dequantisation, which pays from a few sequences on (four: 1440 against 798), and twice the tensor rate in prefill.  Embedding and head keep their type.  An engine
-        that serves this model captures its decode graphs anew at its next step."""
+        that serves this model captures its decode graphs anew at its next step; with tensor parallelism
+        every rank converts, between the same two steps."""
         from ..ops.quant import untile_weight
         for L in self.layers:
             for name in ("wqkv", "wo", "wgu", "wdown"):
