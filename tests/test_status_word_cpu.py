@@ -1,6 +1,5 @@
 """The kernels' status word is seen by host threads only once it is ready."""
 import threading
-import time
 
 import torch
 
@@ -9,12 +8,13 @@ from axonml_b200 import _native as N
 
 def test_threads_see_one_word_and_only_when_it_is_ready(monkeypatch):
     monkeypatch.setattr(N, "_STATUS", {})
-    made, ready = [], threading.Event()
+    made, begun, go, ready = [], threading.Event(), threading.Event(), threading.Event()
 
-    def slow(dev):
+    def slow(dev):                                        # the fill of the word, and the wait for it
         t = torch.zeros(4, dtype=torch.int32)
         made.append(t)
-        time.sleep(0.2)                                   # the fill of the word, and the wait for it
+        begun.set()
+        assert go.wait(60)
         ready.set()
         return t
     monkeypatch.setattr(N, "_new_status_word", slow)
@@ -27,11 +27,13 @@ def test_threads_see_one_word_and_only_when_it_is_ready(monkeypatch):
     threads = [threading.Thread(target=use) for _ in range(8)]
     for t in threads:
         t.start()
-    time.sleep(0.05)
-    assert not N._STATUS                                  # nothing is published before it is ready
+    assert begun.wait(60)
+    published = dict(N._STATUS)
+    go.set()
     for t in threads:
         t.join()
-    assert len(made) == 1 and all(w is made[0] for w in got) and not any(early)
+    assert not published                                  # nothing is seen before it is ready
+    assert len(got) == 8 and len(made) == 1 and all(w is made[0] for w in got) and not any(early)
     assert N.status_word("cpu") is made[0]
 
 
